@@ -475,6 +475,101 @@ int kvx_qk_norm_rope(void* qkv, int64_t stride_b, int64_t stride_t, int32_t B, i
                      const float* cos, const float* sin, int32_t table_rows, int32_t input_pos,
                      void* stream);
 
+/* Rotary position encoding of a ragged batch, in place: every token at a position of its own. Query and key heads x of D values, normalised first where
+ * weights are given (as kvx_rmsnorm_rows, a head a row), then the pairs (a, b) of their first rotary_dim values become (a cos - b sin, b cos + a sin):
+ * a, b = x[j], x[j + rotary_dim / 2], or interleaved x[2 j], x[2 j + 1], j < rotary_dim / 2, with the angles of row positions[t] of the tables. All of it
+ * in fp32, rounded once (kvx_qk_norm_rope rounds the normalised head before it is rotated). Tokens whose position is negative or behind the
+ * tables' last row are left as they are (padding), value heads always.
+ * qkv: bf16 or fp16 (elem_dtype KVX_KV_BF16 / KVX_KV_F16) (tokens, (Hq + 2 Hkv) * D) by token stride. cos / sin: fp32 (table_rows, rotary_dim / 2).
+ * positions: int32 (tokens). D in {64, 128, 256}; rotary_dim a multiple of 16, at most D. No counterpart in the reference. */
+typedef struct kvx_rotary_args {
+  void* qkv;
+  int64_t stride_t, tokens;
+  int32_t Hq, Hkv, D, rotary_dim, interleaved, elem_dtype, table_rows;
+  float eps;
+  const float* q_weight; /* (D) norm weights, or both NULL */
+  const float* k_weight;
+  const float* cos;
+  const float* sin;
+  const int32_t* positions;
+} kvx_rotary_args;
+int kvx_rotary(const kvx_rotary_args* args, void* stream);
+
+/* ---- paged cache: rows of any sequence in pages of a common pool ----------------------------- */
+
+/* A pool of pages. Page p holds page_size K and V rows of each KV head: rows at k + p * k_stride_page + h * k_stride_h + i * k_stride_t, with the types and
+ * row layouts of enum kvx_kv_dtype (strides in elements, of codes in bytes), and for codes their scale and zero point at [p * qs_stride_page +
+ * h * qs_stride_h + i] (the arrays share strides, places contiguous). A slot is p * page_size + i. The pages of a sequence, in order, are a row of a block
+ * table: token t of sequence b lies in page block_table[b * bt_stride_b + t / page_size] at place t % page_size. page_size: a power of two from 16
+ * to 1024. Pointers 16-byte aligned; strides of whole 16 bytes. Offsets of pages may pass 32 bits. The reference has contiguous caches only. */
+typedef struct kvx_pages {
+  int32_t num_pages, page_size, Hkv, D, kv_dtype;
+  void* k;
+  int64_t k_stride_page, k_stride_h, k_stride_t;
+  void* v;
+  int64_t v_stride_page, v_stride_h, v_stride_t;
+  float* k_scale;
+  int32_t* k_zp;
+  float* v_scale;
+  int32_t* v_zp;
+  int64_t qs_stride_page, qs_stride_h;
+} kvx_pages;
+
+/* Write `tokens` new rows: row t of key and value, (tokens, Hkv, D) of the store's element type by strides, to slot slots[t] (int64), quantised on the way in
+ * as kvx_quantize_rows does where the pages hold codes. A negative slot, or one behind the pool's last, is no slot: the row is dropped (padding). Two rows
+ * of one call with the same slot: one of them is stored, or parts of each. */
+typedef struct kvx_paged_write_args {
+  kvx_pages pages;
+  int64_t tokens;
+  const void* key;
+  int64_t key_stride_t, key_stride_h;
+  const void* value;
+  int64_t value_stride_t, value_stride_h;
+  const int64_t* slots;
+} kvx_paged_write_args;
+int kvx_paged_write(const kvx_paged_write_args* args, void* stream);
+
+/* Rows of sequences back, dequantised where the pages hold codes: key / value, (B, Hkv, length, D) of the store's element type by strides, get the first
+ * min(lens[b], length) rows of sequence b, and zeros behind them. Rows of pages that the pool does not have, and of tokens behind
+ * max_pages * page_size, are zeros too. */
+typedef struct kvx_paged_read_args {
+  kvx_pages pages;
+  int32_t B, length, max_pages;
+  const int32_t* block_table; /* (B, max_pages) */
+  int64_t bt_stride_b;
+  const int32_t* lens; /* (B) */
+  void* key;
+  int64_t key_stride_b, key_stride_h, key_stride_t;
+  void* value;
+  int64_t value_stride_b, value_stride_h, value_stride_t;
+} kvx_paged_read_args;
+int kvx_paged_read(const kvx_paged_read_args* args, void* stream);
+
+/* Attention of one new token a sequence over its first lens[b] rows (its own among them): o = softmax(sm_scale q K^T) V and, if lse is given, the base-2
+ * log-sum-exp, fp32 (B, Hq) contiguous. q, o: (B, Hq, D) of the store's element type by strides; Hq / Hkv at most 16. Rows of codes stand for
+ * (code - zp) * scale, not rounded to 16 bits in between. lens[b] is taken between 0 and max_pages * page_size; tokens in pages that the pool
+ * does not have are left out. A sequence without tokens gets zeros and -inf. Rows behind lens[b] may hold anything, infinities and NaN included.
+ * The lengths are read on the device alone, so a captured call may be replayed with others. Work is dealt out to a fixed number of workgroups by the
+ * lengths' sum, in shares of whole 128 tokens, whatever their distribution; results do not depend on anything but the arguments and that number.
+ * workspace: kvx_paged_decode_workspace_bytes(), contents do not matter; calls that may overlap need one each. */
+typedef struct kvx_paged_decode_args {
+  kvx_pages pages;
+  int32_t B, Hq, max_pages;
+  float sm_scale;
+  const void* q;
+  int64_t q_stride_b, q_stride_h;
+  const int32_t* block_table; /* (B, max_pages) */
+  int64_t bt_stride_b;
+  const int32_t* lens; /* (B) */
+  void* o;
+  int64_t o_stride_b, o_stride_h;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+} kvx_paged_decode_args;
+int kvx_paged_decode(const kvx_paged_decode_args* args, void* stream);
+size_t kvx_paged_decode_workspace_bytes(const kvx_paged_decode_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -110,6 +110,63 @@ class BlockQuantArgs(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    """struct kvx_rotary_args"""
+
+    _fields_ = [
+        ("qkv", c_void_p), ("stride_t", c_int64), ("tokens", c_int64),
+        ("Hq", c_int32), ("Hkv", c_int32), ("D", c_int32), ("rotary_dim", c_int32), ("interleaved", c_int32), ("elem_dtype", c_int32), ("table_rows", c_int32),
+        ("eps", c_float),
+        ("q_weight", c_void_p), ("k_weight", c_void_p), ("cos", c_void_p), ("sin", c_void_p), ("positions", c_void_p),
+    ]
+
+
+class Pages(ctypes.Structure):
+    """struct kvx_pages"""
+
+    _fields_ = [
+        ("num_pages", c_int32), ("page_size", c_int32), ("Hkv", c_int32), ("D", c_int32), ("kv_dtype", c_int32),
+        ("k", c_void_p), ("k_stride_page", c_int64), ("k_stride_h", c_int64), ("k_stride_t", c_int64),
+        ("v", c_void_p), ("v_stride_page", c_int64), ("v_stride_h", c_int64), ("v_stride_t", c_int64),
+        ("k_scale", c_void_p), ("k_zp", c_void_p), ("v_scale", c_void_p), ("v_zp", c_void_p),
+        ("qs_stride_page", c_int64), ("qs_stride_h", c_int64),
+    ]
+
+
+class PagedWriteArgs(ctypes.Structure):
+    """struct kvx_paged_write_args"""
+
+    _fields_ = [
+        ("pages", Pages), ("tokens", c_int64),
+        ("key", c_void_p), ("key_stride_t", c_int64), ("key_stride_h", c_int64),
+        ("value", c_void_p), ("value_stride_t", c_int64), ("value_stride_h", c_int64),
+        ("slots", c_void_p),
+    ]
+
+
+class PagedReadArgs(ctypes.Structure):
+    """struct kvx_paged_read_args"""
+
+    _fields_ = [
+        ("pages", Pages), ("B", c_int32), ("length", c_int32), ("max_pages", c_int32),
+        ("block_table", c_void_p), ("bt_stride_b", c_int64), ("lens", c_void_p),
+        ("key", c_void_p), ("key_stride_b", c_int64), ("key_stride_h", c_int64), ("key_stride_t", c_int64),
+        ("value", c_void_p), ("value_stride_b", c_int64), ("value_stride_h", c_int64), ("value_stride_t", c_int64),
+    ]
+
+
+class PagedDecodeArgs(ctypes.Structure):
+    """struct kvx_paged_decode_args"""
+
+    _fields_ = [
+        ("pages", Pages), ("B", c_int32), ("Hq", c_int32), ("max_pages", c_int32), ("sm_scale", c_float),
+        ("q", c_void_p), ("q_stride_b", c_int64), ("q_stride_h", c_int64),
+        ("block_table", c_void_p), ("bt_stride_b", c_int64), ("lens", c_void_p),
+        ("o", c_void_p), ("o_stride_b", c_int64), ("o_stride_h", c_int64),
+        ("lse", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 # every symbol include/kvx.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "kvx_version": (ctypes.c_int, []),
@@ -152,6 +209,11 @@ SYMBOLS = {
     "kvx_swiglu_rows": (ctypes.c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p]),
     "kvx_qk_norm_rope": (ctypes.c_int, [c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p,
                                         ctypes.c_float, c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
+    "kvx_rotary": (ctypes.c_int, [POINTER(RotaryArgs), c_void_p]),
+    "kvx_paged_write": (ctypes.c_int, [POINTER(PagedWriteArgs), c_void_p]),
+    "kvx_paged_read": (ctypes.c_int, [POINTER(PagedReadArgs), c_void_p]),
+    "kvx_paged_decode": (ctypes.c_int, [POINTER(PagedDecodeArgs), c_void_p]),
+    "kvx_paged_decode_workspace_bytes": (c_size_t, [POINTER(PagedDecodeArgs)]),
 }
 
 _lib = None

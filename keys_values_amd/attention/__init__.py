@@ -4,6 +4,7 @@ from .ops import (  # noqa: F401
     get_device_info,
     get_load_error,
     is_available,
+    paged_decode,
     sdpa_decode,
     sdpa_prefill,
     sdpa_prefill_fused,

@@ -150,6 +150,27 @@ def decode_core(
     return _lib.host().decode(query, key, value, scale, return_weights, return_lse, quant, num_splits, scratch_splits)
 
 
+def paged_decode(
+    query: torch.Tensor,
+    key_pages: torch.Tensor,
+    value_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    lens: torch.Tensor,
+    scale: float,
+    return_lse: bool = False,
+    quant: Optional[QuantState] = None,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Attention of one new token a sequence over a paged cache (see ``kvcache.paged`` for the layout of pages and table):
+    query (B, Hq, D), sequences of ``lens`` (B,) tokens each, the new one among them, in the pages of ``block_table``
+    (B, max_pages). Both are int32 and stay on the device: a captured call may be replayed with other lengths and tables.
+    Returns ``(out (B, Hq, D), lse (B, Hq) fp32 base 2 or None)``; a sequence without tokens gets zeros and -inf.
+
+    Group sizes 1 to 16 for every store and head size. Pages of codes (``quant`` given) stand for ``(code - zero point) * scale``: what
+    ``decode_core`` rounds to the query's type before it multiplies is not rounded here. Rows of the pages behind a
+    sequence's end may hold anything."""
+    return _lib.host().paged_decode(query, key_pages, value_pages, block_table, lens, scale, return_lse, quant)
+
+
 # ---- the reference's entry points (keys_values/attention/flashinfer_ops.py:193-440) --------------
 
 

@@ -12,6 +12,7 @@
 // allocator per call, on the caller's stream, and goes back to it when the call returns: nothing outlives a call, and
 // calls from several threads or streams share nothing. Python objects are read with the interpreter lock held; allocation
 // and launch run without it (`unlocked`).
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
@@ -47,6 +48,12 @@ struct Lib {
 #undef X
   decltype(&::kvx_cache_write_first) kvx_cache_write_first = nullptr;  // libraries from before it bind too
   decltype(&::kvx_sdpa_prefill_first) kvx_sdpa_prefill_first = nullptr;  // likewise: the two calls it stands for
+  // the operators of a paged cache: likewise
+  decltype(&::kvx_rotary) kvx_rotary = nullptr;
+  decltype(&::kvx_paged_write) kvx_paged_write = nullptr;
+  decltype(&::kvx_paged_read) kvx_paged_read = nullptr;
+  decltype(&::kvx_paged_decode) kvx_paged_decode = nullptr;
+  decltype(&::kvx_paged_decode_workspace_bytes) kvx_paged_decode_workspace_bytes = nullptr;
   bool bound = false;
 } lib;
 
@@ -115,6 +122,20 @@ void require_args(Py_ssize_t n, Py_ssize_t want, const char* who) {
 void require_gpu(const at::Tensor& t) {
   if (!t.is_cuda())
     raise(PyExc_RuntimeError, "keys_values_amd: tensor on %s; the HIP kernels need a ROCm device and there is no CPU fallback", t.device().str().c_str());
+}
+
+void require_together(const at::Tensor& first, std::initializer_list<const at::Tensor*> others) {
+  require_gpu(first);
+  for (const at::Tensor* t : others) {
+    if (!t) continue;
+    require_gpu(*t);
+    if (t->device() != first.device())
+      raise(PyExc_ValueError, "tensors on %s and %s: one device is needed", first.device().str().c_str(), t->device().str().c_str());
+  }
+}
+template <typename F>
+void require_entry(F entry, const char* name) {
+  if (!entry) raise(PyExc_ImportError, "the bound library does not export %s", name);
 }
 
 // Attributes of the cache object that are read per call, as interned names.
@@ -922,6 +943,253 @@ PyObject* qk_norm_rope(PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// rotary(qkv, n_head, n_query_groups, head_size, q_weight or None, k_weight or None, eps, cos, sin, positions, interleaved)
+PyObject* rotary(PyObject* const* args, Py_ssize_t n) {
+  require_args(n, 11, "rotary");
+  require_entry(lib.kvx_rotary, "kvx_rotary");
+  const at::Tensor &qkv = tensor(args[0], "qkv"), &cos = tensor(args[7], "cos"), &sin = tensor(args[8], "sin"), &positions = tensor(args[9], "positions");
+  const at::Tensor *qw = opt_tensor(args[4], "q_weight"), *kw = opt_tensor(args[5], "k_weight");
+  require_together(qkv, {&cos, &sin, &positions, qw, kw});
+  const at::ScalarType type = qkv.scalar_type();
+  if (type != at::kBFloat16 && type != at::kHalf)
+    raise(PyExc_NotImplementedError, "qkv.dtype must be torch.bfloat16 or torch.float16, got %s", dtype_name(type).c_str());
+  const int64_t hq = integer(args[1]), hkv = integer(args[2]), d = integer(args[3]);
+  if (hq <= 0 || hkv <= 0 || d <= 0 || hq > INT32_MAX || hkv > INT32_MAX) raise(PyExc_ValueError, "n_head, n_query_groups and head_size must be positive");
+  check_head_size(d);
+  if (qkv.dim() < 2 || qkv.size(-1) != (hq + 2 * hkv) * d || qkv.stride(-1) != 1)
+    raise(PyExc_ValueError, "qkv must be (..., (%lld + 2 * %lld) * %lld) with a contiguous last axis, got shape %s", (long long)hq, (long long)hkv, (long long)d,
+          shape_str(qkv).c_str());
+  // the tokens' axes as one: in place, so a copy would not do
+  int64_t tokens = 1, stride = 0;
+  for (int64_t i = qkv.dim() - 2; i >= 0; --i) {
+    if (qkv.size(i) == 1) continue;
+    if (tokens == 1) stride = qkv.stride(i);
+    else if (qkv.stride(i) != stride * tokens) raise(PyExc_ValueError, "the tokens of qkv must lie at one stride");
+    tokens *= qkv.size(i);
+  }
+  if (positions.scalar_type() != at::kInt || positions.sizes() != qkv.sizes().slice(0, qkv.dim() - 1) || !positions.is_contiguous())
+    raise(PyExc_ValueError, "positions must be contiguous int32 of qkv's leading shape, got %s of shape %s", dtype_name(positions.scalar_type()).c_str(),
+          shape_str(positions).c_str());
+  if (cos.sizes() != sin.sizes() || cos.dim() != 2 || cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat || !cos.is_contiguous() || !sin.is_contiguous() ||
+      cos.size(0) == 0 || cos.size(0) > INT32_MAX)
+    raise(PyExc_ValueError, "cos / sin must be contiguous float32 (positions, rotary_dim / 2) tables of the same shape");
+  if (cos.size(1) == 0 || 2 * cos.size(1) > d || cos.size(1) % 8 != 0)
+    raise(PyExc_NotImplementedError, "a rotary part of %lld values: a multiple of 16 is needed, at most the head size %lld", (long long)(2 * cos.size(1)), (long long)d);
+  for (const at::Tensor* w : {qw, kw})
+    if (w && (w->scalar_type() != at::kFloat || w->dim() != 1 || w->size(0) != d || !w->is_contiguous()))
+      raise(PyExc_ValueError, "norm weights must be float32 of shape (%lld,)", (long long)d);
+  kvx_rotary_args a{};
+  a.qkv = qkv.data_ptr();
+  a.stride_t = stride;
+  a.tokens = tokens;
+  a.Hq = (int32_t)hq;
+  a.Hkv = (int32_t)hkv;
+  a.D = (int32_t)d;
+  a.rotary_dim = (int32_t)(2 * cos.size(1));
+  a.interleaved = truth(args[10]);
+  a.elem_dtype = elem_dtype(type);
+  a.table_rows = (int32_t)cos.size(0);
+  a.eps = (float)real(args[6]);
+  a.q_weight = qw ? (const float*)qw->data_ptr() : nullptr;
+  a.k_weight = kw ? (const float*)kw->data_ptr() : nullptr;
+  a.cos = (const float*)cos.data_ptr();
+  a.sin = (const float*)sin.data_ptr();
+  a.positions = (const int32_t*)positions.data_ptr();
+  const Launch L(qkv);
+  check(unlocked([&] { return lib.kvx_rotary(&a, L.stream); }));
+  Py_RETURN_NONE;
+}
+
+// ---- paged cache -------------------------------------------------------------------------------------------------------------
+
+// The pool behind (num_pages, Hkv, page_size, row) tensors; `state`: the quantiser's, None for plain pages. Rows of `type`, of D values.
+kvx_pages pages_of(const at::Tensor& k, const at::Tensor& v, const Quant* qs, int64_t D, at::ScalarType type) {
+  if (k.dim() != 4 || k.sizes() != v.sizes() || k.stride(3) != 1 || v.stride(3) != 1)
+    raise(PyExc_ValueError, "pages must be (num_pages, n_query_groups, page_size, row) tensors of one shape with contiguous rows, got %s and %s", shape_str(k).c_str(),
+          shape_str(v).c_str());
+  const at::ScalarType want = qs ? at::kByte : type;
+  for (const at::Tensor* t : {&k, &v})
+    if (t->scalar_type() != want)
+      raise(PyExc_NotImplementedError, "pages of dtype %s: %s is needed", dtype_name(t->scalar_type()).c_str(), dtype_name(want).c_str());
+  const bool packed = qs && k.size(3) * 2 == D;
+  if (!packed && k.size(3) != D) raise(PyExc_ValueError, "pages with rows of %lld do not fit head size %lld", (long long)k.size(3), (long long)D);
+  for (int i = 0; i < 4; ++i)
+    if (k.size(i) <= 0 || k.size(i) > INT32_MAX) raise(PyExc_ValueError, "pages of shape %s", shape_str(k).c_str());
+  kvx_pages p{};
+  p.num_pages = (int32_t)k.size(0);
+  p.Hkv = (int32_t)k.size(1);
+  p.page_size = (int32_t)k.size(2);
+  p.D = (int32_t)D;
+  p.kv_dtype = qs ? quant_dtype(packed ? 4 : 8, type) : elem_dtype(type);
+  p.k = k.data_ptr();
+  p.k_stride_page = k.stride(0);
+  p.k_stride_h = k.stride(1);
+  p.k_stride_t = k.stride(2);
+  p.v = v.data_ptr();
+  p.v_stride_page = v.stride(0);
+  p.v_stride_h = v.stride(1);
+  p.v_stride_t = v.stride(2);
+  if (qs) {
+    for (const at::Tensor* t : {&qs->ks, &qs->kz, &qs->vs, &qs->vz})
+      if (t->dim() != 3 || t->sizes() != k.sizes().slice(0, 3) || t->stride(2) != 1 || t->strides() != qs->ks.strides())
+        raise(PyExc_ValueError, "quantisation state must be (num_pages, n_query_groups, page_size) arrays sharing strides, last axis contiguous");
+    if (qs->ks.scalar_type() != at::kFloat || qs->vs.scalar_type() != at::kFloat || qs->kz.scalar_type() != at::kInt || qs->vz.scalar_type() != at::kInt)
+      raise(PyExc_ValueError, "quantisation state must be float32 scales and int32 zero points");
+    p.k_scale = (float*)qs->ks.data_ptr();
+    p.k_zp = (int32_t*)qs->kz.data_ptr();
+    p.v_scale = (float*)qs->vs.data_ptr();
+    p.v_zp = (int32_t*)qs->vz.data_ptr();
+    p.qs_stride_page = qs->ks.stride(0);
+    p.qs_stride_h = qs->ks.stride(1);
+  }
+  return p;
+}
+void require_state(const at::Tensor& first, const std::optional<Quant>& qs) {
+  if (qs) require_together(first, {&qs->ks, &qs->kz, &qs->vs, &qs->vz});
+}
+
+// block_table int32 (B, max_pages) with a contiguous last axis, lens int32 (B) contiguous
+void check_sequences(const at::Tensor& table, const at::Tensor& lens) {
+  if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(1) == 0 || table.stride(1) != 1)
+    raise(PyExc_ValueError, "block_table must be an int32 (sequences, pages) tensor with a contiguous last axis, got %s of shape %s", dtype_name(table.scalar_type()).c_str(),
+          shape_str(table).c_str());
+  if (lens.scalar_type() != at::kInt || lens.dim() != 1 || lens.size(0) != table.size(0) || !lens.is_contiguous())
+    raise(PyExc_ValueError, "lens must be a contiguous int32 tensor of shape (%lld,), got %s of shape %s", (long long)table.size(0), dtype_name(lens.scalar_type()).c_str(),
+          shape_str(lens).c_str());
+  if (table.size(0) > INT32_MAX || table.size(1) > INT32_MAX) raise(PyExc_ValueError, "block_table of shape %s", shape_str(table).c_str());
+}
+
+// paged_write(key, value, key_pages, value_pages, slots, quant or None)
+PyObject* paged_write(PyObject* const* args, Py_ssize_t n) {
+  require_args(n, 6, "paged_write");
+  require_entry(lib.kvx_paged_write, "kvx_paged_write");
+  const at::Tensor &key = tensor(args[0], "key"), &value = tensor(args[1], "value"), &kp = tensor(args[2], "key_pages"), &vp = tensor(args[3], "value_pages"),
+                   &slots = tensor(args[4], "slots");
+  std::optional<Quant> qs;
+  if (args[5] != Py_None) qs.emplace(args[5]);
+  require_together(key, {&value, &kp, &vp, &slots});
+  require_state(key, qs);
+  const at::ScalarType type = key.scalar_type();
+  if (type != at::kBFloat16 && type != at::kHalf)
+    raise(PyExc_NotImplementedError, "key.dtype must be torch.bfloat16 or torch.float16, got %s", dtype_name(type).c_str());
+  if (value.scalar_type() != type) raise(PyExc_ValueError, "key and value must have one dtype");
+  if (key.dim() != 3 || key.sizes() != value.sizes() || key.stride(2) != 1 || value.stride(2) != 1)
+    raise(PyExc_ValueError, "key and value must be (tokens, n_query_groups, head_size) with contiguous rows, got %s and %s", shape_str(key).c_str(), shape_str(value).c_str());
+  check_head_size(key.size(2));
+  if (slots.scalar_type() != at::kLong || slots.dim() != 1 || slots.size(0) != key.size(0) || !slots.is_contiguous())
+    raise(PyExc_ValueError, "slots must be a contiguous int64 tensor of shape (%lld,), got %s of shape %s", (long long)key.size(0), dtype_name(slots.scalar_type()).c_str(),
+          shape_str(slots).c_str());
+  kvx_paged_write_args a{};
+  a.pages = pages_of(kp, vp, qs ? &*qs : nullptr, key.size(2), type);
+  if (a.pages.Hkv != key.size(1)) raise(PyExc_ValueError, "%lld heads of key do not fit pages of %d", (long long)key.size(1), a.pages.Hkv);
+  a.tokens = key.size(0);
+  a.key = key.data_ptr();
+  a.key_stride_t = key.size(0) > 1 ? key.stride(0) : 0;
+  a.key_stride_h = key.size(1) > 1 ? key.stride(1) : 0;
+  a.value = value.data_ptr();
+  a.value_stride_t = key.size(0) > 1 ? value.stride(0) : 0;
+  a.value_stride_h = key.size(1) > 1 ? value.stride(1) : 0;
+  a.slots = (const int64_t*)slots.data_ptr();
+  const Launch L(key);
+  check(unlocked([&] { return lib.kvx_paged_write(&a, L.stream); }));
+  Py_RETURN_NONE;
+}
+
+PyObject* two(const at::Tensor& x, const at::Tensor& y) {
+  PyObject* r = PyTuple_New(2);
+  if (!r) throw PyRaised{};
+  PyTuple_SET_ITEM(r, 0, wrap(x));
+  PyTuple_SET_ITEM(r, 1, wrap(y));
+  return r;
+}
+
+// paged_read(key_pages, value_pages, block_table, lens, length, head_size, dtype, quant or None) -> (key, value)
+PyObject* paged_read(PyObject* const* args, Py_ssize_t n) {
+  require_args(n, 8, "paged_read");
+  require_entry(lib.kvx_paged_read, "kvx_paged_read");
+  const at::Tensor &kp = tensor(args[0], "key_pages"), &vp = tensor(args[1], "value_pages"), &table = tensor(args[2], "block_table"), &lens = tensor(args[3], "lens");
+  std::optional<Quant> qs;
+  if (args[7] != Py_None) qs.emplace(args[7]);
+  require_together(kp, {&vp, &table, &lens});
+  require_state(kp, qs);
+  const int64_t length = integer(args[4]), d = integer(args[5]);
+  if (length < 0 || length > INT32_MAX) raise(PyExc_ValueError, "length = %lld", (long long)length);
+  check_head_size(d);
+  if (!THPDtype_Check(args[6])) raise(PyExc_TypeError, "dtype must be a torch.dtype, not %s", Py_TYPE(args[6])->tp_name);
+  const at::ScalarType type = ((THPDtype*)args[6])->scalar_type;
+  if (type != at::kBFloat16 && type != at::kHalf) raise(PyExc_NotImplementedError, "rows of torch.bfloat16 or torch.float16, not %s", dtype_name(type).c_str());
+  kvx_paged_read_args a{};
+  a.pages = pages_of(kp, vp, qs ? &*qs : nullptr, d, type);
+  check_sequences(table, lens);
+  a.B = (int32_t)table.size(0);
+  a.length = (int32_t)length;
+  a.max_pages = (int32_t)table.size(1);
+  a.block_table = (const int32_t*)table.data_ptr();
+  a.bt_stride_b = table.size(0) > 1 ? table.stride(0) : 0;
+  a.lens = (const int32_t*)lens.data_ptr();
+  const Launch L(kp);
+  at::Tensor key, value;
+  check(unlocked([&] {
+    key = L.empty({a.B, a.pages.Hkv, length, d}, type);
+    value = L.empty({a.B, a.pages.Hkv, length, d}, type);
+    a.key = key.data_ptr();
+    a.key_stride_b = a.value_stride_b = a.pages.Hkv * length * d;
+    a.key_stride_h = a.value_stride_h = length * d;
+    a.key_stride_t = a.value_stride_t = d;
+    a.value = value.data_ptr();
+    return lib.kvx_paged_read(&a, L.stream);
+  }));
+  return two(key, value);
+}
+
+// paged_decode(query, key_pages, value_pages, block_table, lens, scale, return_lse, quant or None) -> (out (B, Hq, D), lse (B, Hq) or None)
+PyObject* paged_decode(PyObject* const* args, Py_ssize_t n) {
+  require_args(n, 8, "paged_decode");
+  require_entry(lib.kvx_paged_decode, "kvx_paged_decode");
+  const at::Tensor &q = tensor(args[0], "query"), &kp = tensor(args[1], "key_pages"), &vp = tensor(args[2], "value_pages"), &table = tensor(args[3], "block_table"),
+                   &lens = tensor(args[4], "lens");
+  std::optional<Quant> qs;
+  if (args[7] != Py_None) qs.emplace(args[7]);
+  require_together(q, {&kp, &vp, &table, &lens});
+  require_state(q, qs);
+  const at::ScalarType type = q.scalar_type();
+  if (type != at::kBFloat16 && type != at::kHalf)
+    raise(PyExc_NotImplementedError, "query.dtype must be torch.bfloat16 or torch.float16, got %s", dtype_name(type).c_str());
+  if (q.dim() != 3 || q.stride(2) != 1) raise(PyExc_ValueError, "query must be (sequences, n_head, head_size) with contiguous rows, got shape %s", shape_str(q).c_str());
+  check_head_size(q.size(2));
+  kvx_paged_decode_args a{};
+  a.pages = pages_of(kp, vp, qs ? &*qs : nullptr, q.size(2), type);
+  check_heads(q.size(1), a.pages.Hkv);
+  check_sequences(table, lens);
+  if (table.size(0) != q.size(0)) raise(PyExc_ValueError, "block_table has %lld rows for %lld sequences", (long long)table.size(0), (long long)q.size(0));
+  a.B = (int32_t)q.size(0);
+  a.Hq = (int32_t)q.size(1);
+  a.max_pages = (int32_t)table.size(1);
+  a.sm_scale = (float)real(args[5]);
+  a.q = q.data_ptr();
+  a.q_stride_b = q.size(0) > 1 ? q.stride(0) : 0;
+  a.q_stride_h = q.size(1) > 1 ? q.stride(1) : 0;
+  a.block_table = (const int32_t*)table.data_ptr();
+  a.bt_stride_b = table.size(0) > 1 ? table.stride(0) : 0;
+  a.lens = (const int32_t*)lens.data_ptr();
+  const bool want_lse = truth(args[6]);
+  const Launch L(q);
+  at::Tensor out, lse;
+  check(unlocked([&] {
+    out = L.empty({a.B, a.Hq, a.pages.D}, type);
+    if (want_lse) lse = L.empty({a.B, a.Hq}, at::kFloat);
+    a.o = out.data_ptr();
+    a.o_stride_b = (int64_t)a.Hq * a.pages.D;
+    a.o_stride_h = a.pages.D;
+    a.lse = (float*)data(lse);
+    const at::Tensor ws = L.scratch(lib.kvx_paged_decode_workspace_bytes(&a));
+    a.workspace = data(ws);
+    a.workspace_bytes = ws.defined() ? (size_t)ws.numel() : 0;
+    return lib.kvx_paged_decode(&a, L.stream);
+  }));
+  return two(out, lse);
+}
+
 // ---- module -------------------------------------------------------------------------------------------------------------------
 
 // bind(path, KvxError, torch.OutOfMemoryError): take the entry points from the library at `path` (already loaded by ctypes: the same handle)
@@ -939,6 +1207,9 @@ PyObject* bind(PyObject* const* args, Py_ssize_t n) {
 #undef X
   l.kvx_cache_write_first = (decltype(l.kvx_cache_write_first))dlsym(h, "kvx_cache_write_first");
   l.kvx_sdpa_prefill_first = (decltype(l.kvx_sdpa_prefill_first))dlsym(h, "kvx_sdpa_prefill_first");
+#define X(name) l.name = (decltype(l.name))dlsym(h, #name);
+  X(kvx_rotary) X(kvx_paged_write) X(kvx_paged_read) X(kvx_paged_decode) X(kvx_paged_decode_workspace_bytes)
+#undef X
   l.bound = true;
   lib = l;
   Py_XSETREF(kvx_error, Py_NewRef(args[1]));
@@ -967,7 +1238,7 @@ PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void (*)(void))entry<bind, false>, METH_FASTCALL, nullptr},
     METHOD(prefill), METHOD(score_sum), METHOD(decode), METHOD(check_qkv), METHOD(cache_write), METHOD(cache_write_first), METHOD(prefill_first), METHOD(cache_update), METHOD(cache_decode_step),
     METHOD(quantize_blocks), METHOD(dequantize_blocks), METHOD(dequantize_rows), METHOD(rmsnorm), METHOD(add_rmsnorm),
-    METHOD(swiglu), METHOD(qk_norm_rope), {nullptr, nullptr, 0, nullptr}};
+    METHOD(swiglu), METHOD(qk_norm_rope), METHOD(rotary), METHOD(paged_write), METHOD(paged_read), METHOD(paged_decode), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Native host path of the kernels (see csrc/host.cpp).", -1, methods};
 
 }  // namespace

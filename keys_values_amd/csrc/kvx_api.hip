@@ -7,6 +7,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <initializer_list>
+
 #include "prefill_merge.h"
 
 namespace kvx {
@@ -474,6 +476,128 @@ int kvx_qk_norm_rope(void* qkv, int64_t stride_b, int64_t stride_t, int32_t B, i
                   (!q_weight || (aligned16(q_weight) && aligned16(k_weight))),
               KVX_ERR_INVALID, "kvx_qk_norm_rope: pointers and strides must keep 16-byte alignment");
   return launch_qk_norm_rope(qkv, stride_b, stride_t, B, num, Hq, Hkv, D, q_weight, k_weight, eps, cos, sin, input_pos, (hipStream_t)stream);
+}
+
+int kvx_rotary(const kvx_rotary_args* a, void* stream) {
+  KVX_REQUIRE(a != nullptr, KVX_ERR_INVALID, "kvx_rotary: args is NULL");
+  KVX_REQUIRE(a->tokens >= 0 && a->Hq > 0 && a->Hkv > 0, KVX_ERR_INVALID, "kvx_rotary: tokens=%lld Hq=%d Hkv=%d", (long long)a->tokens, a->Hq, a->Hkv);
+  KVX_REQUIRE(a->D == 64 || a->D == 128 || a->D == 256, KVX_ERR_UNSUPPORTED, "kvx_rotary: head size %d not in {64, 128, 256}", a->D);
+  KVX_REQUIRE(a->elem_dtype == KVX_KV_BF16 || a->elem_dtype == KVX_KV_F16, KVX_ERR_UNSUPPORTED, "kvx_rotary: unknown elem_dtype %d", a->elem_dtype);
+  KVX_REQUIRE(a->rotary_dim > 0 && a->rotary_dim <= a->D && a->rotary_dim % 16 == 0, KVX_ERR_UNSUPPORTED,
+              "kvx_rotary: rotary_dim=%d must be a multiple of 16, at most the head size %d", a->rotary_dim, a->D);
+  KVX_REQUIRE(a->Hq <= 65535 && a->Hkv <= 65535 && a->tokens <= INT32_MAX, KVX_ERR_UNSUPPORTED, "kvx_rotary: %lld tokens of %d + %d heads", (long long)a->tokens,
+              a->Hq, a->Hkv);
+  KVX_REQUIRE(a->table_rows > 0, KVX_ERR_INVALID, "kvx_rotary: table_rows=%d", a->table_rows);
+  if (a->tokens == 0) return KVX_OK;
+  KVX_REQUIRE(a->qkv && a->cos && a->sin && a->positions, KVX_ERR_INVALID, "kvx_rotary: NULL pointer");
+  KVX_REQUIRE((a->q_weight == nullptr) == (a->k_weight == nullptr), KVX_ERR_INVALID, "kvx_rotary: give both norm weights or none");
+  KVX_REQUIRE(a->tokens == 1 || a->stride_t >= ((int64_t)a->Hq + a->Hkv) * a->D, KVX_ERR_INVALID, "kvx_rotary: token stride %lld shorter than the query and key heads",
+              (long long)a->stride_t);
+  KVX_REQUIRE(aligned16(a->qkv) && aligned16(a->cos) && aligned16(a->sin) && mult8(a->stride_t) && (!a->q_weight || (aligned16(a->q_weight) && aligned16(a->k_weight))),
+              KVX_ERR_INVALID, "kvx_rotary: pointers and the token stride must keep 16-byte alignment");
+  return launch_rotary(*a, (hipStream_t)stream);
+}
+
+static int check_pages(const kvx_pages& p, const char* who) {
+  KVX_REQUIRE(p.num_pages > 0 && p.Hkv > 0, KVX_ERR_INVALID, "%s: num_pages=%d Hkv=%d must be positive", who, p.num_pages, p.Hkv);
+  KVX_REQUIRE(p.page_size >= 16 && p.page_size <= 1024 && (p.page_size & (p.page_size - 1)) == 0, KVX_ERR_UNSUPPORTED,
+              "%s: page_size=%d must be a power of two from 16 to 1024", who, p.page_size);
+  KVX_REQUIRE(kv_valid(p.kv_dtype), KVX_ERR_UNSUPPORTED, "%s: unknown kv_dtype %d", who, p.kv_dtype);
+  KVX_REQUIRE(p.D == 64 || p.D == 128 || p.D == 256, KVX_ERR_UNSUPPORTED, "%s: head size %d not in {64, 128, 256}", who, p.D);
+  KVX_REQUIRE(p.Hkv <= 65535, KVX_ERR_UNSUPPORTED, "%s: Hkv=%d beyond 65535", who, p.Hkv);
+  KVX_REQUIRE(p.k && p.v, KVX_ERR_INVALID, "%s: k and v must be given", who);
+  const bool plain = kv_is_plain(p.kv_dtype);
+  const int64_t whole = plain ? 8 : 16;  // 16 bytes
+  const int row = kv_is_u4(p.kv_dtype) ? p.D / 2 : p.D;
+  const int64_t strides[] = {p.k_stride_page, p.k_stride_h, p.k_stride_t, p.v_stride_page, p.v_stride_h, p.v_stride_t};
+  for (int64_t s : strides)
+    KVX_REQUIRE(s >= 0 && s % whole == 0, KVX_ERR_INVALID, "%s: strides of the pages must be whole 16 bytes, got %lld elements", who, (long long)s);
+  KVX_REQUIRE(aligned16(p.k) && aligned16(p.v), KVX_ERR_INVALID, "%s: k and v must be 16-byte aligned", who);
+  // a page's rows are addressed from its first by 32-bit byte offsets
+  KVX_REQUIRE(p.k_stride_t >= row && p.v_stride_t >= row && p.k_stride_t <= (1 << 19) && p.v_stride_t <= (1 << 19), KVX_ERR_UNSUPPORTED,
+              "%s: slot strides %lld, %lld outside [%d, 2^19]", who, (long long)p.k_stride_t, (long long)p.v_stride_t, row);
+  if (!plain) {
+    KVX_REQUIRE(p.k_scale && p.k_zp && p.v_scale && p.v_zp, KVX_ERR_INVALID, "%s: pages of codes need scales and zero points", who);
+    KVX_REQUIRE(aligned16(p.k_scale) && aligned16(p.k_zp) && aligned16(p.v_scale) && aligned16(p.v_zp) && p.qs_stride_page >= 0 && p.qs_stride_h >= 0 &&
+                    p.qs_stride_page % 4 == 0 && p.qs_stride_h % 4 == 0,
+                KVX_ERR_INVALID, "%s: scales and zero points must be 16-byte aligned with strides that are multiples of 4", who);
+  }
+  return KVX_OK;
+}
+
+static int check_rows(const void* p, const char* name, const char* who, std::initializer_list<int64_t> strides) {
+  bool ok = p && aligned16(p);
+  for (int64_t s : strides) ok = ok && mult8(s);
+  KVX_REQUIRE(ok, KVX_ERR_INVALID, "%s: %s must be given, 16-byte aligned, with strides that are multiples of 8 elements", who, name);
+  return KVX_OK;
+}
+
+int kvx_paged_write(const kvx_paged_write_args* a, void* stream) {
+  static const char who[] = "kvx_paged_write";
+  KVX_REQUIRE(a != nullptr, KVX_ERR_INVALID, "%s: args is NULL", who);
+  int rc = check_pages(a->pages, who);
+  if (rc != KVX_OK) return rc;
+  KVX_REQUIRE(a->tokens >= 0, KVX_ERR_INVALID, "%s: tokens=%lld", who, (long long)a->tokens);
+  KVX_REQUIRE(a->tokens <= INT32_MAX, KVX_ERR_UNSUPPORTED, "%s: %lld tokens", who, (long long)a->tokens);
+  if (a->tokens == 0) return KVX_OK;
+  KVX_REQUIRE(a->slots, KVX_ERR_INVALID, "%s: slots must be given", who);
+  if ((rc = check_rows(a->key, "key", who, {a->key_stride_t, a->key_stride_h})) != KVX_OK) return rc;
+  if ((rc = check_rows(a->value, "value", who, {a->value_stride_t, a->value_stride_h})) != KVX_OK) return rc;
+  return launch_paged_write(*a, (hipStream_t)stream);
+}
+
+static int check_sequences(const char* who, int32_t B, int32_t max_pages, const int32_t* block_table, int64_t bt_stride_b, const int32_t* lens, int32_t page_size) {
+  KVX_REQUIRE(B >= 0 && max_pages > 0, KVX_ERR_INVALID, "%s: B=%d max_pages=%d", who, B, max_pages);
+  KVX_REQUIRE(B <= 65535 && (int64_t)max_pages * page_size < ((int64_t)1 << 30), KVX_ERR_UNSUPPORTED, "%s: B=%d beyond 65535 or tables of %d pages beyond 2^30 tokens",
+              who, B, max_pages);
+  KVX_REQUIRE(B == 0 || (block_table && lens && bt_stride_b >= 0), KVX_ERR_INVALID, "%s: block_table and lens must be given", who);
+  return KVX_OK;
+}
+
+int kvx_paged_read(const kvx_paged_read_args* a, void* stream) {
+  static const char who[] = "kvx_paged_read";
+  KVX_REQUIRE(a != nullptr, KVX_ERR_INVALID, "%s: args is NULL", who);
+  int rc = check_pages(a->pages, who);
+  if (rc != KVX_OK) return rc;
+  if ((rc = check_sequences(who, a->B, a->max_pages, a->block_table, a->bt_stride_b, a->lens, a->pages.page_size)) != KVX_OK) return rc;
+  KVX_REQUIRE(a->length >= 0, KVX_ERR_INVALID, "%s: length=%d", who, a->length);
+  KVX_REQUIRE(a->length < (1 << 30), KVX_ERR_UNSUPPORTED, "%s: length=%d beyond 2^30", who, a->length);
+  if (a->B == 0 || a->length == 0) return KVX_OK;
+  if ((rc = check_rows(a->key, "key", who, {a->key_stride_b, a->key_stride_h, a->key_stride_t})) != KVX_OK) return rc;
+  if ((rc = check_rows(a->value, "value", who, {a->value_stride_b, a->value_stride_h, a->value_stride_t})) != KVX_OK) return rc;
+  return launch_paged_read(*a, (hipStream_t)stream);
+}
+
+static int check_paged_decode(const kvx_paged_decode_args* a) {
+  static const char who[] = "kvx_paged_decode";
+  KVX_REQUIRE(a != nullptr, KVX_ERR_INVALID, "%s: args is NULL", who);
+  int rc = check_pages(a->pages, who);
+  if (rc != KVX_OK) return rc;
+  if ((rc = check_sequences(who, a->B, a->max_pages, a->block_table, a->bt_stride_b, a->lens, a->pages.page_size)) != KVX_OK) return rc;
+  KVX_REQUIRE(a->Hq > 0 && a->Hq % a->pages.Hkv == 0, KVX_ERR_INVALID, "%s: Hq=%d must be a positive multiple of Hkv=%d", who, a->Hq, a->pages.Hkv);
+  KVX_REQUIRE(a->Hq / a->pages.Hkv <= 16, KVX_ERR_UNSUPPORTED, "%s: %d query heads per KV head (at most 16)", who, a->Hq / a->pages.Hkv);
+  const int64_t units = (int64_t)a->B * a->pages.Hkv * (((int64_t)a->max_pages * a->pages.page_size + 127) / 128);
+  KVX_REQUIRE(units < ((int64_t)1 << 30), KVX_ERR_UNSUPPORTED, "%s: %d sequences of %d pages, %d KV heads: beyond 2^30 shares of 128 tokens", who, a->B, a->max_pages,
+              a->pages.Hkv);
+  KVX_REQUIRE(a->sm_scale > 0.0f, KVX_ERR_INVALID, "%s: sm_scale must be positive", who);
+  return KVX_OK;
+}
+
+int kvx_paged_decode(const kvx_paged_decode_args* a, void* stream) {
+  int rc = check_paged_decode(a);
+  if (rc != KVX_OK) return rc;
+  if (a->B == 0) return KVX_OK;
+  if ((rc = check_rows(a->q, "q", "kvx_paged_decode", {a->q_stride_b, a->q_stride_h})) != KVX_OK) return rc;
+  if ((rc = check_rows(a->o, "o", "kvx_paged_decode", {a->o_stride_b, a->o_stride_h})) != KVX_OK) return rc;
+  const size_t need = paged_decode_workspace(*a);
+  KVX_REQUIRE(need == 0 || (aligned16(a->workspace) && a->workspace && a->workspace_bytes >= need), KVX_ERR_WORKSPACE,
+              "kvx_paged_decode: workspace of %zu bytes, 16-byte aligned, is needed, got %zu", need, a->workspace ? a->workspace_bytes : (size_t)0);
+  return launch_paged_decode(*a, (hipStream_t)stream);
+}
+
+size_t kvx_paged_decode_workspace_bytes(const kvx_paged_decode_args* a) {
+  if (check_paged_decode(a) != KVX_OK || a->B == 0) return 0;
+  return paged_decode_workspace(*a);
 }
 
 }  // extern "C"

@@ -111,6 +111,11 @@ int launch_add_rmsnorm_rows(const void* x, int64_t x_rs, const void* delta, int6
 int launch_swiglu_rows(const void* gate_up, int64_t g_rs, void* out, int64_t o_rs, int64_t rows, int dim, hipStream_t st);
 int launch_qk_norm_rope(void* qkv, int64_t sb, int64_t stt, int B, int num, int Hq, int Hkv, int D, const float* qw, const float* kw,
                         float eps, const float* cos_t, const float* sin_t, int input_pos, hipStream_t st);
+int launch_rotary(const kvx_rotary_args& a, hipStream_t st);
+int launch_paged_write(const kvx_paged_write_args& a, hipStream_t st);
+int launch_paged_read(const kvx_paged_read_args& a, hipStream_t st);
+int launch_paged_decode(const kvx_paged_decode_args& a, hipStream_t st);
+size_t paged_decode_workspace(const kvx_paged_decode_args& a);
 
 // Number of compute units of the current device (cached).
 int num_cus();

@@ -34,6 +34,7 @@ class PrefillConfig:
     rope_base: float = 1.0e6
     norm_eps: float = 1.0e-6
     norm_qk: bool = True
+    rope_scaling: Optional[ops.RopeScaling] = None  # angles for contexts beyond the trained one
 
 
 # Qwen3-4B architecture numbers
@@ -119,7 +120,7 @@ class LongContextPrefillModel:
         # the layer's dense part on a second stream
         self.caches = [H2OKVCache(params, max_chunk_size=chunk_size, quantized=quantized, device=self.device, overlap_select=True)
                        for _ in range(cfg.n_layer)]
-        self.cos, self.sin = ops.rope_tables(max_context, cfg.head_size, cfg.rope_base, self.device)
+        self.cos, self.sin = ops.rope_tables(max_context, cfg.head_size, cfg.rope_base, self.device, scaling=cfg.rope_scaling)
         self.input_pos = 0
 
     def reset(self):
