@@ -26,7 +26,7 @@
 namespace kvx {
 namespace {
 
-constexpr int NT = 256, WAVES = 4, UNIT = 128;  // keys of a unit: a block of 32 a wavefront
+constexpr int NT = 256, WAVES = 4, UNIT = 128;  // keys of a step: a block of 32 a wavefront
 constexpr float kLowest = -3.4028235e38f;       // running maximum before the first key
 typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 
@@ -37,29 +37,31 @@ struct PagedParams {
   int cap;          // tokens of a table's pages
   int Gr;           // query heads per KV head
   int workgroups;
+  int unit;         // log2 of the keys of a unit
+  uint32_t k_page, v_page, q_page;  // bytes from page to page of K, V and the quantiser's arrays
+  int by_pair;      // part_of goes by pairs, which are fewer, else by workgroups
   float* part_o;    // (2 workgroups, Gr, D)
   float* part_ml;   // (2 workgroups, Gr, 2): maximum and sum
-  int* part_of;     // (workgroups, 2): the pair whose first partial the workgroup left, and how many the pair has
+  int* part_of;     // by pairs: the workgroup that left a pair's first partial; by workgroups: the pair; and how many partials the pair has, 0: none
 };
 
-__device__ __forceinline__ int units_of(int len, int cap) { return max(1, (min(max(len, 0), cap) + UNIT - 1) / UNIT); }
+__device__ __forceinline__ int units_of(int len, int cap, int unit) { return max(1, (min(max(len, 0), cap) + (1 << unit) - 1) >> unit); }
 
-// Inclusive sum over the lanes of a wavefront.
+// Inclusive sum over the lanes of a wavefront, on the vector ALU.
 __device__ __forceinline__ int scan(int x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(x, off, 64);
-    if (lane >= off) x += y;
-  }
-  return x;
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);  // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);  // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);  // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 to the odd rows
+  return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 to the upper half
 }
 
 // The shares of `total` units: workgroup w begins with unit first(w).
 struct Shares {
-  int each, rest;
-  __device__ __forceinline__ Shares(int total, int workgroups) : each(total / workgroups), rest(total - each * workgroups) {}
-  __device__ __forceinline__ int first(int w) const { return w * each + min(w, rest); }
+  int workgroups, each, rest;
+  __device__ __forceinline__ Shares(int total, int n) : workgroups(n), each(total / n), rest(total - each * n) {}
+  __device__ __forceinline__ int first(int w) const { return min(w, workgroups) * each + min(w, rest); }
   __device__ __forceinline__ int owner(int unit) const {
     const int big = rest * (each + 1);
     return unit < big ? unit / (each + 1) : rest + (unit - big) / each;
@@ -74,15 +76,14 @@ struct Rows {
   static constexpr int KR = U4 ? NL4 : (CODES ? D / 64 : KJ);                         // 16-byte loads per key of K
   static constexpr int VB = U4 ? DPL / 2 : DPL * ES;                                  // bytes per key of V
   static constexpr int VW = (VB + 3) / 4;
+  // state: lane l has the scale of key l (l < 32) or the zero point of key l - 32
   struct K {
     u32x4_t w[2][KR];
-    f32x4_t scale[2];
-    i32x4_t zp[2];
+    uint32_t state;
   };
   struct V {
     uint32_t w[8][VW];
-    f32x4_t scale[2];
-    i32x4_t zp[2];
+    uint32_t state;
   };
   // first d of the 8 that lane group kg supplies to matrix instruction e of the first product
   __device__ __forceinline__ static int kslice(int e, int kg) {
@@ -131,80 +132,271 @@ struct Rows {
   }
 };
 
+// What a block's keys are multiplied by and what is added to them, of a lane's keys: 4 kg + i of either tile. A lane loads the scale or the zero point of one key
+// (lanes 0 - 31 and 32 - 63), makes of it what is wanted, and the keys' values change hands through LDS of the wavefront's own. Loaded as they are used, by 16 lanes each,
+// they took as many cycles of the address units as 4-bit rows of 128, 32 registers on the way, and their conversions a third of the loop.
+struct State {
+  f32x4_t scale[2], zp[2];
+  __device__ __forceinline__ State(float* lds, float mine, int lane, int kg) {
+    lds[lane] = mine;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int gi = 0; gi < 2; ++gi) {
+      scale[gi] = *(const f32x4_t*)(lds + 16 * gi + 4 * kg);
+      zp[gi] = *(const f32x4_t*)(lds + 32 + 16 * gi + 4 * kg);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+};
+
+// Maximum over the wavefront, in every lane.
+__device__ __forceinline__ float max_lanes(float x) {
+  auto step = [](float v, auto ctrl) {
+    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, 0xf, 0xf, false)));
+  };
+  x = step(x, std::integral_constant<int, 0x128>{});  // row_ror:8
+  x = step(x, std::integral_constant<int, 0x124>{});  // row_ror:4
+  x = step(x, std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
+  x = step(x, std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
+  return max_halves(max_row_pairs(x));
+}
+// Sum over the four lane groups of a column.
+__device__ __forceinline__ float sum_groups(float x) {
+  const u32pair_t r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
 template <typename T>
 __device__ __forceinline__ T once(const void* p) { return __builtin_nontemporal_load((const T*)p); }
 
 // Wavefronts a SIMD: as many as the registers of a block of keys allow.
-template <int D, int KV>
-constexpr int waves_per_simd() { return D == 256 && kv_is_plain(KV) ? 1 : D == 256 ? 2 : 3; }
+constexpr int waves_per_simd(int D, bool codes) { return D == 256 ? (codes ? 2 : 1) : D == 128 ? (codes ? 3 : 3) : (codes ? 4 : 4); }
 
 template <int D, int KV>
-__global__ __launch_bounds__(NT, (waves_per_simd<D, KV>())) void paged_decode_kernel(const PagedParams p) {
+__global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged_decode_kernel(const PagedParams p) {
   using R = Rows<D, KV>;
   constexpr bool F16 = R::F16, CODES = R::CODES, U4 = R::U4, P16 = F16 || CODES;  // P16: weights and operands in fp16
   constexpr int KJ = R::KJ, DPL = R::DPL, ES = R::ES;
   // The running maximum moves when a logit exceeds it by kTop. Weights in fp16 are kept below 2^15, and brought to 2^7 when it moves: what is a normal number
   // there goes down to 2^-21 of the largest then, and what is not zero to 2^-32.
   constexpr float kTop = P16 ? 15.0f : 8.0f, kBias = P16 ? 7.0f : 0.0f;
+  // The part of a weight that its 16 bits drop is a second operand where outputs have as many bits: the rounding of weights would be as large as theirs.
+  constexpr bool FINE = F16;
   constexpr int RS = D + 4;  // floats of a head's row in LDS: heads in different banks
   __shared__ __align__(16) float red[WAVES][16][RS];
-  __shared__ float red_m[WAVES][16], red_l[WAVES][16], weight[WAVES][16], fin[2][16];
+  __shared__ __align__(16) float state[WAVES][2][64];
+  __shared__ float red_m[WAVES][16], red_l[WAVES][16];
 
   const kvx_pages& pg = p.a.pages;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, kg = lane >> 4;
   const int B = p.a.B, Hkv = pg.Hkv, w = blockIdx.x, mask = pg.page_size - 1;
   const int* const lens = p.a.lens;
 
-  // ---- this workgroup's units: every wavefront finds them for itself
-  int b, begin_b, unit, end;  // sequence, its first unit, the next unit, the end of the share
-  Shares shares(0, 1);
-  {
-    const int per = (B + 63) / 64;
-    int mine = 0;
-    for (int i = 0; i < per; ++i)
-      if (lane * per + i < B) mine += units_of(lens[lane * per + i], p.cap);
-    const int upto = scan(mine), total = __builtin_amdgcn_readlane(upto, 63) * Hkv;
-    shares = Shares(total, p.workgroups);
-    unit = shares.first(w);
-    end = shares.first(w + 1);
-    const int at = __builtin_ctzll(__ballot(upto * Hkv > unit) | (1ull << 63));
-    b = at * per;
-    begin_b = __builtin_amdgcn_readlane(upto - mine, at) * Hkv;
-    for (; b < B - 1; ++b) {
-      const int n = units_of(lens[b], p.cap) * Hkv;
-      if (begin_b + n > unit) break;
-      begin_b += n;
-    }
+  // ---- this workgroup's units: every wavefront finds them for itself, 64 sequences at a time
+  const int windows = (B + 63) / 64;
+  auto window = [&](int i) { return 64 * i + lane < B ? lens[64 * i + lane] : -1; };
+  auto units_in = [&](int len, int i) { return 64 * i + lane < B ? units_of(len, p.cap, p.unit) : 0; };
+  int lane_len = 0, mine = 0;  // lane_len: of sequence (b & ~63) + lane
+  for (int i = 0; i < windows; ++i) {
+    lane_len = window(i);
+    mine += units_in(lane_len, i);
   }
-  if (tid == 0) p.part_of[2 * w + 1] = 0;
+  const int total = __builtin_amdgcn_readlane(scan(mine), 63) * Hkv;
+  const Shares shares(total, p.workgroups);
+  int unit = shares.first(w);  // the next unit
+  const int end = shares.first(w + 1);
+  if (tid == 0 && p.part_of && !p.by_pair) p.part_of[2 * w + 1] = 0;
+  if (unit >= end) return;
+  int b, begin_b;  // its sequence, and the sequence's first unit
+  for (int i = 0, before = 0;; ++i) {
+    if (windows > 1) lane_len = window(i);
+    mine = units_in(lane_len, i);
+    const int upto = before + scan(mine);
+    const unsigned long long behind = __ballot(upto * Hkv > unit);
+    if (behind) {
+      const int at = __builtin_ctzll(behind);
+      b = 64 * i + at;
+      begin_b = __builtin_amdgcn_readlane(upto - mine, at) * Hkv;
+      break;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+
+  // A stretch of a pair's units. The next one's first rows are on their way while this one's results are joined.
+  struct Stretch {
+    int b, h, begin, units, first, n, k_begin, k_end;
+  };
+  auto take = [&] {
+    Stretch s;
+    const int len = min(max(__builtin_amdgcn_readlane(lane_len, b & 63), 0), p.cap);
+    s.b = b;
+    s.units = units_of(len, p.cap, p.unit);
+    s.h = (unit - begin_b) / s.units;
+    s.begin = begin_b + s.h * s.units;
+    s.first = unit - s.begin;
+    s.n = min(s.units - s.first, end - unit);
+    s.k_begin = s.first << p.unit;
+    s.k_end = min(len, (s.first + s.n) << p.unit);
+    unit += s.n;
+    if (unit == begin_b + s.units * Hkv) {
+      begin_b = unit;
+      ++b;
+      if ((b & 63) == 0 && b < B) lane_len = window(b >> 6);
+    }
+    return s;
+  };
 
   const uint32_t k_rowb = (uint32_t)pg.k_stride_t * ES, v_rowb = (uint32_t)pg.v_stride_t * ES;
   const uint32_t k_lane = (uint32_t)m * k_rowb + (U4 && D == 64 ? 8 : 16) * kg, v_lane = 4 * kg * v_rowb + (uint32_t)m * R::VB;
 
-  while (unit < end) {
-    const int len = min(max(lens[b], 0), p.cap), units = units_of(len, p.cap);
-    const int h = (unit - begin_b) / units, begin = begin_b + h * units, first = unit - begin, n_units = min(units - first, end - unit);
-    const int k_begin = first * UNIT, k_end = min(len, (first + n_units) * UNIT);
+  // ---- rows of a block of 32 keys. Lane 2 j + gi holds the page of half gi of the wavefront's block j (of 32 at a time). A page that the pool does not have is
+  // read as page 0, and its keys are masked behind. Keys behind the end lie in the same pages, or masked ones.
+  struct Tiles {
+    int page0, page1;  // no arrays: a lane that picks one of them would send them through memory
+    bool ok0, ok1;
+    __device__ __forceinline__ int page(bool upper) const {
+      const int a = page0, b = page1;
+      return upper ? b : a;
+    }
+    __device__ __forceinline__ bool ok(bool upper) const {
+      const bool a = ok0, b = ok1;
+      return upper ? b : a;
+    }
+  };
+  Stretch at;       // the stretch whose rows are read
+  int lane_page;
+  const uint8_t *k_head, *v_head;
+  const char *k_state, *v_state;
+  auto pages_of = [&](const Stretch& s, int j) {
+    return p.a.block_table[s.b * p.a.bt_stride_b + min((s.k_begin + 32 * wave + (j + (lane >> 1)) * UNIT + 16 * (lane & 1)) >> p.shift, p.a.max_pages - 1)];
+  };
+  auto tiles = [&](int j) {
+    if (j > 0 && (j & 31) == 0) {
+      lane_page = pages_of(at, j);
+      asm volatile("" : "+v"(lane_page));  // waited for here, not in every pass
+    }
+    Tiles t;
+    const int page0 = __builtin_amdgcn_readlane(lane_page, 2 * (j & 31)), page1 = __builtin_amdgcn_readlane(lane_page, 2 * (j & 31) + 1);
+    t.ok0 = (uint32_t)page0 < (uint32_t)pg.num_pages;
+    t.ok1 = (uint32_t)page1 < (uint32_t)pg.num_pages;
+    t.page0 = t.ok0 ? page0 : 0;
+    t.page1 = t.ok1 ? page1 : 0;
+    return t;
+  };
+  auto load_state = [&](const char* base, int chunk, const Tiles& t) {
+    const uint32_t page = t.page(lane & 16), place = (chunk + (lane & 16)) & mask;
+    return once<uint32_t>(base + ((uint64_t)page * p.q_page + place * 4u));
+  };
+  auto load_k = [&](typename R::K& r, int chunk, const Tiles& t) {
+#pragma unroll
+    for (int gi = 0; gi < 2; ++gi) {
+      const uint8_t* base = k_head + (uint64_t)(uint32_t)t.page(gi) * p.k_page;
+      const uint32_t off = (uint32_t)((chunk + 16 * gi) & mask) * k_rowb + k_lane;
+#pragma unroll
+      for (int x = 0; x < R::KR; ++x) {
+        if constexpr (U4 && D == 64) {
+          const u32x2_t y = once<u32x2_t>(base + off);
+          r.w[gi][x] = u32x4_t{y[0], y[1], 0u, 0u};
+        } else {
+          r.w[gi][x] = once<u32x4_t>(base + off + 64 * x);
+        }
+      }
+    }
+    if constexpr (CODES) r.state = load_state(k_state, chunk, t);
+  };
+  auto load_v = [&](typename R::V& r, int chunk, const Tiles& t) {
+    if constexpr (CODES) r.state = load_state(v_state, chunk, t);
+#pragma unroll
+    for (int gi = 0; gi < 2; ++gi) {
+      const uint8_t* base = v_head + (uint64_t)(uint32_t)t.page(gi) * p.v_page;
+      const uint32_t off = (uint32_t)((chunk + 16 * gi) & mask) * v_rowb + v_lane;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* row = base + (off + (uint32_t)i * v_rowb);
+        uint32_t(&x)[R::VW] = r.w[4 * gi + i];
+        if constexpr (R::VB >= 16) {
+#pragma unroll
+          for (int y = 0; y < R::VB / 16; ++y) {
+            const u32x4_t z = once<u32x4_t>(row + 16 * y);
+            x[4 * y] = z[0]; x[4 * y + 1] = z[1]; x[4 * y + 2] = z[2]; x[4 * y + 3] = z[3];
+          }
+        } else if constexpr (R::VB == 8) {
+          const u32x2_t z = once<u32x2_t>(row);
+          x[0] = z[0]; x[1] = z[1];
+        } else if constexpr (R::VB == 4) {
+          x[0] = once<uint32_t>(row);
+        } else {
+          x[0] = (uint32_t)once<uint16_t>(row);
+        }
+      }
+    }
+  };
+  // Queries, B operands of the first product: head m (zero beyond the group)
+  auto load_q = [&](u32x4_t (&q)[KJ], const Stretch& s) {
+    const uint16_t* row = (const uint16_t*)p.a.q + s.b * p.a.q_stride_b + (int64_t)(s.h * p.Gr + min(m, p.Gr - 1)) * p.a.q_stride_h;
+#pragma unroll
+    for (int e = 0; e < KJ; ++e) q[e] = *(const u32x4_t*)(row + R::kslice(e, kg));
+  };
+  typename R::K k;
+  typename R::V v;
+  u32x4_t qb[KJ];
+  Tiles t;
+  auto start = [&](const Stretch& s, int page) {
+    at = s;
+    lane_page = page;
+    k_head = (const uint8_t*)pg.k + s.h * pg.k_stride_h * ES;
+    v_head = (const uint8_t*)pg.v + s.h * pg.v_stride_h * ES;
+    if constexpr (CODES) {
+      const int64_t q = s.h * pg.qs_stride_h + m;
+      k_state = (const char*)((lane < 32 ? (const uint32_t*)pg.k_scale : (const uint32_t*)pg.k_zp) + q);
+      v_state = (const char*)((lane < 32 ? (const uint32_t*)pg.v_scale : (const uint32_t*)pg.v_zp) + q);
+    }
+    t = tiles(0);
+    load_q(qb, s);
+    const int chunk = s.k_begin + 32 * wave;
+    if (chunk < s.k_end) {
+      load_k(k, chunk, t);
+      load_v(v, chunk, t);
+    }
+  };
+  {
+    const Stretch s = take();
+    start(s, pages_of(s, 0));
+  }
 
-    // ---- queries: B operands of the first product, head m (zero beyond the group)
-    u32x4_t qb[KJ];
+  for (bool again = false;; again = true) {
+    const Stretch now = at;
+    const bool more = unit < end;
+    Stretch next = now;
+    int next_page = 0;
+    if (more) {
+      next = take();
+      next_page = pages_of(next, 0);
+    }
+
     float qsum = 0.0f, to_logit = p.c;
 #pragma unroll
-    for (int e = 0; e < KJ; ++e) {
-      qb[e] = u32x4_t{0u, 0u, 0u, 0u};
-      if (m < p.Gr) qb[e] = *(const u32x4_t*)((const uint16_t*)p.a.q + b * p.a.q_stride_b + (int64_t)(h * p.Gr + m) * p.a.q_stride_h + R::kslice(e, kg));
-    }
+    for (int e = 0; e < KJ; ++e)
+      if (m >= p.Gr) qb[e] = u32x4_t{0u, 0u, 0u, 0u};
     if constexpr (CODES) {
-      float top = 0.0f;
+      auto largest = [&](bool finite) {  // of the group's queries
+        float top = 0.0f;
 #pragma unroll
-      for (int e = 0; e < KJ; ++e)
+        for (int e = 0; e < KJ; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(elem_lo<F16>(qb[e][i])), fabsf(elem_hi<F16>(qb[e][i]))));
-      top = max_halves(max_row_pairs(top));
-      // 2^x that brings the largest to [2^14, 2^15); zeros, infinities and NaN stay
-      const int ex = (int)(__float_as_uint(top) >> 23), up = ex == 0 || ex == 255 ? 127 : min(268 - ex, 253);
+          for (int i = 0; i < 4; ++i) {
+            const float x0 = fabsf(elem_lo<F16>(qb[e][i])), x1 = fabsf(elem_hi<F16>(qb[e][i]));
+            top = fmaxf(top, finite && !(x0 < INFINITY) ? 0.0f : x0);
+            top = fmaxf(top, finite && !(x1 < INFINITY) ? 0.0f : x1);
+          }
+        return max_lanes(top);
+      };
+      float top = largest(false);
+      if (!(top < INFINITY)) top = largest(true);
+      // 2^x that brings it to [2^14, 2^15)
+      const int ex = (int)(__float_as_uint(top) >> 23), up = ex == 0 ? 127 : min(268 - ex, 253);
       const float by = __uint_as_float((uint32_t)up << 23);
-      to_logit = __uint_as_float((uint32_t)(254 - up) << 23) * p.c;
+      to_logit = __uint_as_float((uint32_t)(254 - up) << 23) * p.c * 0x1p24f;
 #pragma unroll
       for (int e = 0; e < KJ; ++e) {
         float x[8];
@@ -222,112 +414,41 @@ __global__ __launch_bounds__(NT, (waves_per_simd<D, KV>())) void paged_decode_ke
           qb[e] = u32x4_t{pack_pair<true>(x[0], x[1]), pack_pair<true>(x[2], x[3]), pack_pair<true>(x[4], x[5]), pack_pair<true>(x[6], x[7])};
         }
       }
-      qsum = sum_halves([](float v) {
-        const u32pair_t r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-      }(qsum));
+      qsum = -sum_groups(qsum) * 0x1p-24f;
     }
 
     f32x4_t acc[DPL];
 #pragma unroll
     for (int t = 0; t < DPL; ++t) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     float m_run = kLowest, l_run = 0.0f;
-    float corr = 0.0f, unit_v = 0x1p-126f, per_v = 0x1p126f;  // codes: sum of c w' + w (zp - c); the unit of the scales, and its inverse
+    // codes: sum of w (zp - c), sum of w' in every row, the unit of the scales, and its inverse
+    float corr = 0.0f, unit_v = 0x1p-126f, per_v = 0x1p126f;
+    f32x4_t wsum = {0.0f, 0.0f, 0.0f, 0.0f};
 
-    // ---- rows of a block of 32 keys. The pages of its two halves come by scalar loads; a page that the pool does not have is read as page 0, and its keys are
-    // masked behind. Keys behind the end lie in the same pages, or masked ones.
-    struct Tiles {
-      int page[2];
-    };
-    const auto table = (const int __attribute__((address_space(4)))*)(uintptr_t)(p.a.block_table + b * p.a.bt_stride_b);
-    auto pages = [&](int chunk) {
-      Tiles t;
-#pragma unroll
-      for (int gi = 0; gi < 2; ++gi) t.page[gi] = table[min((chunk + 16 * gi) >> p.shift, p.a.max_pages - 1)];
-      return t;
-    };
-    auto there = [&](int page) { return (uint32_t)page < (uint32_t)pg.num_pages; };
-    auto load_k = [&](typename R::K& r, int chunk, const Tiles& t) {
-#pragma unroll
-      for (int gi = 0; gi < 2; ++gi) {
-        const int64_t page = there(t.page[gi]) ? t.page[gi] : 0;
-        const uint8_t* base = (const uint8_t*)pg.k + (page * pg.k_stride_page + h * pg.k_stride_h) * ES;
-        const int place = (chunk + 16 * gi) & mask;
-        const uint32_t off = (uint32_t)place * k_rowb + k_lane;
-#pragma unroll
-        for (int x = 0; x < R::KR; ++x) {
-          if constexpr (U4 && D == 64) {
-            const u32x2_t y = once<u32x2_t>(base + off);
-            r.w[gi][x] = u32x4_t{y[0], y[1], 0u, 0u};
-          } else {
-            r.w[gi][x] = once<u32x4_t>(base + off + 64 * x);
-          }
-        }
-        if constexpr (CODES) {
-          const int64_t q = page * pg.qs_stride_page + h * pg.qs_stride_h + place;
-          r.scale[gi] = once<f32x4_t>((const char*)(pg.k_scale + q) + 16 * kg);
-          r.zp[gi] = once<i32x4_t>((const char*)(pg.k_zp + q) + 16 * kg);
-        }
-      }
-    };
-    auto load_v = [&](typename R::V& r, int chunk, const Tiles& t) {
-#pragma unroll
-      for (int gi = 0; gi < 2; ++gi) {
-        const int64_t page = there(t.page[gi]) ? t.page[gi] : 0;
-        const uint8_t* base = (const uint8_t*)pg.v + (page * pg.v_stride_page + h * pg.v_stride_h) * ES;
-        const int place = (chunk + 16 * gi) & mask;
-        const uint32_t off = (uint32_t)place * v_rowb + v_lane;
-        if constexpr (CODES) {
-          const int64_t q = page * pg.qs_stride_page + h * pg.qs_stride_h + place;
-          r.scale[gi] = once<f32x4_t>((const char*)(pg.v_scale + q) + 16 * kg);
-          r.zp[gi] = once<i32x4_t>((const char*)(pg.v_zp + q) + 16 * kg);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint8_t* row = base + (off + (uint32_t)i * v_rowb);
-          uint32_t(&x)[R::VW] = r.w[4 * gi + i];
-          if constexpr (R::VB >= 16) {
-#pragma unroll
-            for (int y = 0; y < R::VB / 16; ++y) {
-              const u32x4_t z = once<u32x4_t>(row + 16 * y);
-              x[4 * y] = z[0]; x[4 * y + 1] = z[1]; x[4 * y + 2] = z[2]; x[4 * y + 3] = z[3];
-            }
-          } else if constexpr (R::VB == 8) {
-            const u32x2_t z = once<u32x2_t>(row);
-            x[0] = z[0]; x[1] = z[1];
-          } else if constexpr (R::VB == 4) {
-            x[0] = once<uint32_t>(row);
-          } else {
-            x[0] = (uint32_t)once<uint16_t>(row);
-          }
-        }
-      }
-    };
-    auto whole = [&](int chunk, const Tiles& t) { return chunk + 32 <= k_end && there(t.page[0]) && there(t.page[1]); };
-    // key 4 kg + i of tile gi, this lane's, is one of the sequence's
-    auto live = [&](int chunk, const Tiles& t, int gi, int i) { return there(t.page[gi]) && chunk + 16 * gi + 4 * kg + i < k_end; };
-    // logits in log2 units: head m, keys 4 kg + i of the two tiles
-    auto logits = [&](const typename R::K& r, int chunk, const Tiles& t, float (&s)[8]) {
+    auto whole = [&](int chunk) { return chunk + 32 <= now.k_end && t.ok0 && t.ok1; };
+    // key `i` of half gi is one of the sequence's
+    auto live = [&](int chunk, int gi, int i) { return t.ok(gi) && chunk + 16 * gi + i < now.k_end; };
+    // logits in log2 units: head m, keys 4 kg + i of the two halves
+    auto logits = [&](int chunk, float (&s)[8]) {
       f32x4_t x[2];
 #pragma unroll
       for (int gi = 0; gi < 2; ++gi) {
         x[gi] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int e = 0; e < KJ; ++e) x[gi] = mfma_16x16x32<P16>(R::k_operand(r, gi, e), qb[e], x[gi]);
+        for (int e = 0; e < KJ; ++e) x[gi] = mfma_16x16x32<P16>(R::k_operand(k, gi, e), qb[e], x[gi]);
       }
+      if constexpr (CODES) {
+        const State st(state[wave][0], lane < 32 ? __uint_as_float(k.state) * to_logit : (float)(int32_t)k.state, lane, kg);
 #pragma unroll
-      for (int gi = 0; gi < 2; ++gi)
+        for (int i = 0; i < 8; ++i) s[i] = fmaf(st.zp[i >> 2][i & 3], qsum, x[i >> 2][i & 3]) * st.scale[i >> 2][i & 3];
+      } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (CODES) s[4 * gi + i] = fmaf(-(float)r.zp[gi][i], qsum, x[gi][i] * 0x1p24f) * (r.scale[gi][i] * to_logit);
-          else s[4 * gi + i] = x[gi][i] * to_logit;
-        }
-      if (!whole(chunk, t)) {
+        for (int i = 0; i < 8; ++i) s[i] = x[i >> 2][i & 3] * to_logit;
+      }
+      if (!whole(chunk)) {
 #pragma unroll
-        for (int gi = 0; gi < 2; ++gi)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!live(chunk, t, gi, i)) s[4 * gi + i] = -INFINITY;
+        for (int i = 0; i < 8; ++i)
+          if (!live(chunk, i >> 2, 4 * kg + (i & 3))) s[i] = -INFINITY;
       }
     };
     auto weights = [&](float (&s)[8]) {
@@ -340,7 +461,10 @@ __global__ __launch_bounds__(NT, (waves_per_simd<D, KV>())) void paged_decode_ke
         const float to = moves ? top - kBias : m_run, al = moves ? fast_exp2(m_run - to) : 1.0f;
         m_run = to;
         l_run *= al;
-        corr *= al;
+        if constexpr (CODES) {
+          corr *= al;
+          wsum *= al;
+        }
 #pragma unroll
         for (int t = 0; t < DPL; ++t) acc[t] *= al;
       }
@@ -350,185 +474,200 @@ __global__ __launch_bounds__(NT, (waves_per_simd<D, KV>())) void paged_decode_ke
         l_run += s[i];
       }
     };
-    auto outputs = [&](typename R::V& r, int chunk, const Tiles& t, float (&s)[8]) {
-      if (!whole(chunk, t)) {  // what lies in masked places may be infinite or NaN
+    auto outputs = [&](int chunk, float (&s)[8]) {
+      const bool masked = !whole(chunk);  // what lies in masked places may be infinite or NaN
+      if constexpr (!CODES)
+        if (masked) {
 #pragma unroll
-        for (int gi = 0; gi < 2; ++gi)
+          for (int i = 0; i < 8; ++i)
+            if (!live(chunk, i >> 2, 4 * kg + (i & 3))) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!live(chunk, t, gi, i)) {
-              if constexpr (CODES) {
-                r.scale[gi][i] = 0.0f;
-                r.zp[gi][i] = 0;
-              } else {
-#pragma unroll
-                for (int y = 0; y < R::VW; ++y) r.w[4 * gi + i][y] = 0u;
-              }
+              for (int y = 0; y < R::VW; ++y) v.w[i][y] = 0u;
             }
-      }
-      if constexpr (CODES) {
-        float top = r.scale[0][0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) top = fmaxf(top, r.scale[i >> 2][i & 3]);
-        if (__any(top > unit_v)) {
-          top = max_halves(max_row_pairs(top));
-          if (top > unit_v) {
-            const int ex = min((int)(__float_as_uint(top) >> 23) + 1, 253);
-            const float to = __uint_as_float((uint32_t)ex << 23), al = unit_v * __uint_as_float((uint32_t)(254 - ex) << 23);
-            unit_v = to;
-            per_v = __uint_as_float((uint32_t)(254 - ex) << 23);
-            corr *= al;
-#pragma unroll
-            for (int t = 0; t < DPL; ++t) acc[t] *= al;
-          }
         }
-        constexpr int MID = U4 ? 8 : 128;
+      if constexpr (CODES) {
+        constexpr float MID = U4 ? 8.0f : 128.0f;
+        float mine = lane < 32 ? __uint_as_float(v.state) : (float)(int32_t)v.state - MID;
+        if (masked && !live(chunk, (lane >> 4) & 1, m)) mine = 0.0f;
+        const float scale = lane < 32 ? mine : 0.0f;
+        if (__any(scale > unit_v)) {
+          const int ex = min((int)(__float_as_uint(max_lanes(scale)) >> 23) + 1, 253);
+          const float per = __uint_as_float((uint32_t)(254 - ex) << 23), al = unit_v * per;
+          unit_v = __uint_as_float((uint32_t)ex << 23);
+          per_v = per;
+          corr *= al;
+          wsum *= al;
+#pragma unroll
+          for (int t = 0; t < DPL; ++t) acc[t] *= al;
+        }
+        const State st(state[wave][1], lane < 32 ? mine * per_v : mine, lane, kg);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          s[i] *= r.scale[i >> 2][i & 3] * per_v;
-          corr = fmaf(s[i], (float)(r.zp[i >> 2][i & 3] - MID), corr);
+          s[i] *= st.scale[i >> 2][i & 3];
+          corr = fmaf(s[i], st.zp[i >> 2][i & 3], corr);
         }
       }
       const u32x4_t pb = {pack_pair<P16>(s[0], s[1]), pack_pair<P16>(s[2], s[3]), pack_pair<P16>(s[4], s[5]), pack_pair<P16>(s[6], s[7])};
-      if constexpr (CODES) {
-        float sum = 0.0f;
+      const u32x4_t ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+      if constexpr (CODES) wsum = mfma_16x16x32<true>(ones, pb, wsum);
+      if constexpr (FINE) {
+        u32x4_t pl;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += elem_lo<true>(pb[i]) + elem_hi<true>(pb[i]);
-        corr = fmaf(sum, U4 ? 8.0f : 128.0f, corr);
+        for (int i = 0; i < 4; ++i) pl[i] = pack_pair<P16>(s[2 * i] - elem_lo<P16>(pb[i]), s[2 * i + 1] - elem_hi<P16>(pb[i]));
+        if constexpr (CODES) wsum = mfma_16x16x32<true>(ones, pl, wsum);
+#pragma unroll
+        for (int t = 0; t < DPL; ++t) {
+          const u32x4_t x = R::v_operand(v, t);
+          acc[t] = mfma_16x16x32<P16>(x, pl, mfma_16x16x32<P16>(x, pb, acc[t]));
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < DPL; ++t) acc[t] = mfma_16x16x32<P16>(R::v_operand(v, t), pb, acc[t]);
       }
-#pragma unroll
-      for (int t = 0; t < DPL; ++t) acc[t] = mfma_16x16x32<P16>(R::v_operand(r, t), pb, acc[t]);
     };
 
-    int chunk = k_begin + 32 * wave;
-    if (chunk < k_end) {
-      Tiles now = pages(chunk), next = pages(chunk + UNIT);
-      typename R::K k;
-      typename R::V v;
+    int chunk = now.k_begin + 32 * wave;
+    if (chunk < now.k_end) {
       float s[8];
-      load_k(k, chunk, now);
-      load_v(v, chunk, now);
-      for (; chunk + UNIT < k_end; chunk += UNIT) {
-        const Tiles then = pages(chunk + 2 * UNIT);
-        logits(k, chunk, now, s);
+      for (int j = 1; chunk + UNIT < now.k_end; ++j) {
+        const Tiles then = tiles(j);
+        logits(chunk, s);
         __builtin_amdgcn_sched_barrier(0);  // the loads below reuse the registers consumed above
-        load_k(k, chunk + UNIT, next);
+        load_k(k, chunk + UNIT, then);
         __builtin_amdgcn_sched_barrier(0);
         weights(s);
-        outputs(v, chunk, now, s);
+        outputs(chunk, s);
         __builtin_amdgcn_sched_barrier(0);
-        load_v(v, chunk + UNIT, next);
+        load_v(v, chunk + UNIT, then);
         __builtin_amdgcn_sched_barrier(0);
-        now = next;
-        next = then;
+        t = then;
+        chunk += UNIT;
       }
-      logits(k, chunk, now, s);
+      logits(chunk, s);
       weights(s);
-      outputs(v, chunk, now, s);
+      outputs(chunk, s);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) start(next, next_page);
+    __builtin_amdgcn_sched_barrier(0);
 
     // ---- the four wavefronts' results, joined
-    auto over_groups = [](float x) {
-      const u32pair_t r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-      return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-    };
-    const float l = over_groups(l_run);
+    const float l = sum_groups(l_run);
     if constexpr (CODES) {
-      corr = over_groups(corr);
+      corr = fmaf(wsum[0], U4 ? 8.0f : 128.0f, sum_groups(corr));
 #pragma unroll
       for (int t = 0; t < DPL; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[t][i] = (acc[t][i] * (U4 && t < DPL / 2 ? 0x1p20f : 0x1p24f) - corr) * unit_v;
     }
+    if (again) __syncthreads();  // the results before are read
     if (m < p.Gr) {
+      constexpr int RUN = U4 && D == 64 ? 2 : 4;  // values side by side
+      typedef float run_t __attribute__((ext_vector_type(RUN)));
 #pragma unroll
-      for (int t = 0; t < DPL; ++t)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[wave][m][R::dmap(t, 4 * kg + i)] = acc[t][i];
+        for (int t = 0; t < DPL; t += RUN) {
+          run_t x;
+#pragma unroll
+          for (int e = 0; e < RUN; ++e) x[e] = acc[t + e][i];
+          *(run_t*)&red[wave][m][R::dmap(t, 4 * kg + i)] = x;
+        }
       if (kg == 0) {
         red_m[wave][m] = m_run;
         red_l[wave][m] = l;
       }
     }
     __syncthreads();
-    const bool alone = first == 0 && n_units == units;  // the pair is this workgroup's alone
-    const int slot = 2 * w + (first == 0 ? 1 : 0);
-    if (tid < p.Gr) {
-      float top = red_m[0][tid], sum = 0.0f;
+    const bool alone = now.first == 0 && now.n == now.units;  // the pair is this workgroup's alone
+    const int slot = 2 * w + (now.first == 0 ? 1 : 0);
+    auto sums = [&](int g, float (&f)[WAVES], float& top) {
+      top = red_m[0][g];
 #pragma unroll
-      for (int i = 1; i < WAVES; ++i) top = fmaxf(top, red_m[i][tid]);
+      for (int j = 1; j < WAVES; ++j) top = fmaxf(top, red_m[j][g]);
+      float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < WAVES; ++i) {
-        const float f = fast_exp2(red_m[i][tid] - top);
-        weight[i][tid] = f;
-        sum += red_l[i][tid] * f;
+      for (int j = 0; j < WAVES; ++j) {
+        f[j] = fast_exp2(red_m[j][g] - top);
+        sum += red_l[j][g] * f[j];
       }
-      fin[0][tid] = alone ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
-      if (alone) {
-        if (p.a.lse) p.a.lse[(int64_t)b * p.a.Hq + h * p.Gr + tid] = sum == 0.0f ? -INFINITY : top + fast_log2(sum);
-      } else {
-        *(f32x2_t*)(p.part_ml + ((int64_t)slot * p.Gr + tid) * 2) = f32x2_t{top, sum};
-      }
-    }
-    __syncthreads();
+      return sum;
+    };
     for (int i = tid; i < p.Gr * (D / 4); i += NT) {
       const int g = i / (D / 4), d = 4 * (i % (D / 4));
+      float f[WAVES], top;
+      const float sum = sums(g, f, top);
       f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int j = 0; j < WAVES; ++j) x += *(const f32x4_t*)&red[j][g][d] * weight[j][g];
+      for (int j = 0; j < WAVES; ++j) x += *(const f32x4_t*)&red[j][g][d] * f[j];
       if (alone) {
-        x *= fin[0][g];
-        *(u32x2_t*)((uint16_t*)p.a.o + b * p.a.o_stride_b + (int64_t)(h * p.Gr + g) * p.a.o_stride_h + d) = u32x2_t{pack_pair<F16>(x[0], x[1]), pack_pair<F16>(x[2], x[3])};
+        x *= sum == 0.0f ? 0.0f : 1.0f / sum;
+        *(u32x2_t*)((uint16_t*)p.a.o + now.b * p.a.o_stride_b + (int64_t)(now.h * p.Gr + g) * p.a.o_stride_h + d) =
+            u32x2_t{pack_pair<F16>(x[0], x[1]), pack_pair<F16>(x[2], x[3])};
+        if (d == 0 && p.a.lse) p.a.lse[(int64_t)now.b * p.a.Hq + now.h * p.Gr + g] = sum == 0.0f ? -INFINITY : top + fast_log2(sum);
       } else {
         *(f32x4_t*)(p.part_o + ((int64_t)slot * p.Gr + g) * D + d) = x;
+        if (d == 0) *(f32x2_t*)(p.part_ml + ((int64_t)slot * p.Gr + g) * 2) = f32x2_t{top, sum};
       }
     }
-    if (tid == 0 && first == 0 && !alone) {
-      p.part_of[2 * w] = b * Hkv + h;
-      p.part_of[2 * w + 1] = shares.owner(begin + units - 1) - w + 1;
+    if (tid == 0 && p.part_of && now.first == 0 && (p.by_pair || !alone)) {
+      const int pair = now.b * Hkv + now.h, i = 2 * (p.by_pair ? pair : w);
+      p.part_of[i] = p.by_pair ? w : pair;
+      p.part_of[i + 1] = alone ? 0 : shares.owner(now.begin + now.units - 1) - w + 1;
     }
-    __syncthreads();  // LDS is free again
-
-    unit += n_units;
-    if (unit == begin_b + units * Hkv) {
-      begin_b = unit;
-      ++b;
-    }
+    if (!more) break;
   }
 }
 
-// The partials of the pair that workgroup blockIdx.x of the launch above left off in: 256 values of its outputs, four a lane; the wavefronts share the partials.
-template <int D, bool F16>
+// The partials of a pair, joined: 4 LANES of its outputs a workgroup, four a lane; NT / LANES groups of lanes share the partials.
+template <int D, bool F16, int LANES>
 __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedParams p) {
-  const int w = blockIdx.x, n = p.part_of[2 * w + 1];
+  constexpr int GROUPS = NT / LANES, U = 8;  // partials of a group in flight
+  const int at = p.part_of[2 * blockIdx.x], n = p.part_of[2 * blockIdx.x + 1];
   if (n == 0) return;
-  __shared__ __align__(16) float red[WAVES][64][4];
-  __shared__ float red_m[WAVES][64], red_l[WAVES][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.y * 256 + 4 * lane, g = min(i / D, p.Gr - 1), d = i % D;
-  const int pair = p.part_of[2 * w], b = pair / p.a.pages.Hkv, h = pair - b * p.a.pages.Hkv;
+  __shared__ __align__(16) float red[GROUPS][LANES][4];
+  __shared__ float red_m[GROUPS][LANES], red_l[GROUPS][LANES];
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, i = blockIdx.y * 4 * LANES + 4 * lane, g = min(i / D, p.Gr - 1), d = i % D;
+  const int w = p.by_pair ? at : blockIdx.x, pair = p.by_pair ? blockIdx.x : at, b = pair / p.a.pages.Hkv, h = pair - b * p.a.pages.Hkv;
   float top = kLowest, sum = 0.0f;
   f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = wave; s < n; s += WAVES) {
-    const int64_t slot = s == 0 ? 2 * w + 1 : 2 * (w + s);
-    const f32x2_t ml = *(const f32x2_t*)(p.part_ml + (slot * p.Gr + g) * 2);
-    const f32x4_t y = *(const f32x4_t*)(p.part_o + (slot * p.Gr + g) * D + d);
-    const float to = fmaxf(top, ml[0]), al = fast_exp2(top - to), be = fast_exp2(ml[0] - to);
+  for (int s0 = group; s0 < n; s0 += GROUPS * U) {
+    f32x2_t ml[U];
+    f32x4_t y[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = min(s0 + GROUPS * u, n - 1);
+      const int64_t slot = s == 0 ? 2 * w + 1 : 2 * (w + s);
+      ml[u] = *(const f32x2_t*)(p.part_ml + (slot * p.Gr + g) * 2);
+      y[u] = *(const f32x4_t*)(p.part_o + (slot * p.Gr + g) * D + d);
+    }
+    float to = top;
+#pragma unroll
+    for (int u = 0; u < U; ++u) to = fmaxf(to, ml[u][0]);
+    const float al = fast_exp2(top - to);
+    sum *= al;
+    x *= al;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + GROUPS * u >= n) break;
+      const float be = fast_exp2(ml[u][0] - to);
+      sum += ml[u][1] * be;
+      x += y[u] * be;
+    }
     top = to;
-    sum = sum * al + ml[1] * be;
-    x = x * al + y * be;
   }
-  *(f32x4_t*)red[wave][lane] = x;
-  red_m[wave][lane] = top;
-  red_l[wave][lane] = sum;
+  *(f32x4_t*)red[group][lane] = x;
+  red_m[group][lane] = top;
+  red_l[group][lane] = sum;
   __syncthreads();
-  if (wave != 0 || i >= p.Gr * D) return;
+  if (group != 0 || i >= p.Gr * D) return;
   float all = red_m[0][lane];
 #pragma unroll
-  for (int j = 1; j < WAVES; ++j) all = fmaxf(all, red_m[j][lane]);
+  for (int j = 1; j < GROUPS; ++j) all = fmaxf(all, red_m[j][lane]);
   sum = 0.0f;
   x = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int j = 0; j < WAVES; ++j) {
+  for (int j = 0; j < GROUPS; ++j) {
     const float f = fast_exp2(red_m[j][lane] - all);
     sum += red_l[j][lane] * f;
     x += *(const f32x4_t*)red[j][lane] * f;
@@ -543,14 +682,25 @@ PagedParams params_of(const kvx_paged_decode_args& a) {
   p.a = a;
   p.c = a.sm_scale * kLog2e;
   p.shift = __builtin_ctz(a.pages.page_size);
+  const int es = kv_is_plain(a.pages.kv_dtype) ? 2 : 1;
+  p.k_page = (uint32_t)(a.pages.k_stride_page * es);
+  p.v_page = (uint32_t)(a.pages.v_stride_page * es);
+  p.q_page = (uint32_t)(a.pages.qs_stride_page * 4);
   p.cap = a.max_pages << p.shift;
   p.Gr = a.Hq / a.pages.Hkv;
-  const int per_cu = a.pages.D == 256 ? (kv_is_plain(a.pages.kv_dtype) ? 1 : 2) : 3;
-  const int64_t units = (int64_t)a.B * a.pages.Hkv * ((p.cap + UNIT - 1) / UNIT), most = (int64_t)per_cu * num_cus();
+  const int per_cu = waves_per_simd(a.pages.D, !kv_is_plain(a.pages.kv_dtype));  // a workgroup has a wavefront on each
+  // Tables of up to 512 tokens: a pair is a workgroup's, and there is no second launch.
+  p.unit = p.cap <= 4 * UNIT ? 9 : 7;
+  const int64_t pairs = (int64_t)a.B * a.pages.Hkv, units = pairs * ((p.cap + (1 << p.unit) - 1) >> p.unit), cus = num_cus();
+  // One workgroup a compute unit for the only pair: the partials of more take longer to join than they save (one of 100000 tokens, 16 heads of 128: 21.7 us, 33.8
+  // with three).
+  const int64_t most = pairs < per_cu ? pairs * cus : per_cu * cus;
   p.workgroups = (int)(units < most ? units : most);
+  p.by_pair = pairs <= p.workgroups;
   return p;
 }
-bool splits(const PagedParams& p) { return p.cap > UNIT; }
+int64_t pairs_of(const PagedParams& p) { return (int64_t)p.a.B * p.a.pages.Hkv; }
+bool splits(const PagedParams& p) { return p.cap > (1 << p.unit); }
 
 template <int D>
 void launch_head(const PagedParams& p, hipStream_t st) {
@@ -565,9 +715,15 @@ void launch_head(const PagedParams& p, hipStream_t st) {
 #undef KVX_PAGES_CASE
   }
   if (!splits(p)) return;
-  const dim3 grid(p.workgroups, (p.Gr * D + 255) / 256);
-  if (kv_elem_f16(p.a.pages.kv_dtype)) hipLaunchKernelGGL((paged_join_kernel<D, true>), grid, dim3(NT), 0, st, p);
-  else hipLaunchKernelGGL((paged_join_kernel<D, false>), grid, dim3(NT), 0, st, p);
+  const unsigned rows = p.by_pair ? (unsigned)pairs_of(p) : (unsigned)p.workgroups;
+  auto join = [&](auto lanes) {
+    constexpr int LANES = decltype(lanes)::value;
+    const dim3 grid(rows, (p.Gr * D + 4 * LANES - 1) / (4 * LANES));
+    if (kv_elem_f16(p.a.pages.kv_dtype)) hipLaunchKernelGGL((paged_join_kernel<D, true, LANES>), grid, dim3(NT), 0, st, p);
+    else hipLaunchKernelGGL((paged_join_kernel<D, false, LANES>), grid, dim3(NT), 0, st, p);
+  };
+  if (rows <= 64) join(std::integral_constant<int, 16>{});
+  else join(std::integral_constant<int, 64>{});
 }
 
 size_t part_floats(const PagedParams& p) { return (size_t)2 * p.workgroups * p.Gr * p.a.pages.D; }
@@ -576,14 +732,16 @@ size_t part_floats(const PagedParams& p) { return (size_t)2 * p.workgroups * p.G
 
 size_t paged_decode_workspace(const kvx_paged_decode_args& a) {
   const PagedParams p = params_of(a);
-  return 4 * (part_floats(p) + (size_t)4 * p.workgroups * p.Gr + 2 * p.workgroups);
+  return splits(p) ? 4 * (part_floats(p) + (size_t)4 * p.workgroups * p.Gr + 2 * p.workgroups) : 0;
 }
 
 int launch_paged_decode(const kvx_paged_decode_args& a, hipStream_t st) {
   PagedParams p = params_of(a);
-  p.part_o = (float*)a.workspace;
-  p.part_ml = p.part_o + part_floats(p);
-  p.part_of = (int*)(p.part_ml + (size_t)4 * p.workgroups * p.Gr);
+  if (splits(p)) {
+    p.part_o = (float*)a.workspace;
+    p.part_ml = p.part_o + part_floats(p);
+    p.part_of = (int*)(p.part_ml + (size_t)4 * p.workgroups * p.Gr);
+  }
   if (a.pages.D == 256) launch_head<256>(p, st);
   else if (a.pages.D == 128) launch_head<128>(p, st);
   else launch_head<64>(p, st);
