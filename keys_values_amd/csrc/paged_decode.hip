@@ -37,6 +37,7 @@ struct PagedParams {
   int cap;          // tokens of a table's pages
   int Gr;           // query heads per KV head
   int workgroups;
+  int cus;          // compute units
   int unit;         // log2 of the keys of a unit
   uint32_t k_page, v_page, q_page;  // bytes from page to page of K, V and the quantiser's arrays
   int by_pair;      // part_of goes by pairs, which are fewer, else by workgroups
@@ -169,8 +170,8 @@ __device__ __forceinline__ float sum_groups(float x) {
 template <typename T>
 __device__ __forceinline__ T once(const void* p) { return __builtin_nontemporal_load((const T*)p); }
 
-// Wavefronts a SIMD: as many as the registers of a block of keys allow.
-constexpr int waves_per_simd(int D, bool codes) { return D == 256 ? (codes ? 2 : 1) : D == 128 ? (codes ? 3 : 3) : (codes ? 4 : 4); }
+// Wavefronts a SIMD that the registers have to leave room for: plain rows of 256 values take more than half of them.
+constexpr int waves_per_simd(int D, bool codes) { return D == 256 && !codes ? 1 : 2; }
 
 template <int D, int KV>
 __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged_decode_kernel(const PagedParams p) {
@@ -202,7 +203,13 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
     mine += units_in(lane_len, i);
   }
   const int total = __builtin_amdgcn_readlane(scan(mine), 63) * Hkv;
-  const Shares shares(total, p.workgroups);
+  // Workgroups that share the units, of the grid's three a compute unit: all where pairs are short (of up to four units on average; B256, 32 / 8 heads of 128, 50 to 400
+  // tokens: 42.7 us, 44.4 with two a compute unit, 54.2 with one), two elsewhere (64 sequences of 1 to 8192, 28 / 4 heads: 30.9, 33.3 with one, 32.1 with three), and
+  // one, whose partials are the fewest, where pairs are long and rows of 128 bytes and more keep enough of them on their way (16 x 16384, plain rows of 128: 158.3, 162.0
+  // with two, 165.6 with three; but 4-bit rows of 128: 65.7, 53.7 with two).
+  constexpr bool WIDE = D * ES >= (U4 ? 256 : 128);
+  const int pairs = B * Hkv, sharing = total <= 4 * pairs ? p.workgroups : WIDE && total >= 64 * pairs ? p.cus : 2 * p.cus;
+  const Shares shares(total, min(sharing, p.workgroups));
   int unit = shares.first(w);  // the next unit
   const int end = shares.first(w + 1);
   if (tid == 0 && p.part_of && !p.by_pair) p.part_of[2 * w + 1] = 0;
@@ -688,13 +695,13 @@ PagedParams params_of(const kvx_paged_decode_args& a) {
   p.q_page = (uint32_t)(a.pages.qs_stride_page * 4);
   p.cap = a.max_pages << p.shift;
   p.Gr = a.Hq / a.pages.Hkv;
-  const int per_cu = waves_per_simd(a.pages.D, !kv_is_plain(a.pages.kv_dtype));  // a workgroup has a wavefront on each
   // Tables of up to 512 tokens: a pair is a workgroup's, and there is no second launch.
   p.unit = p.cap <= 4 * UNIT ? 9 : 7;
-  const int64_t pairs = (int64_t)a.B * a.pages.Hkv, units = pairs * ((p.cap + (1 << p.unit) - 1) >> p.unit), cus = num_cus();
+  p.cus = num_cus();
   // One workgroup a compute unit for the only pair: the partials of more take longer to join than they save (one of 100000 tokens, 16 heads of 128: 21.7 us, 33.8
   // with three).
-  const int64_t most = pairs < per_cu ? pairs * cus : per_cu * cus;
+  const int64_t per_cu = a.pages.D == 256 ? waves_per_simd(256, !kv_is_plain(a.pages.kv_dtype)) : 3;
+  const int64_t pairs = (int64_t)a.B * a.pages.Hkv, units = pairs * ((p.cap + (1 << p.unit) - 1) >> p.unit), most = p.cus * (pairs < per_cu ? pairs : per_cu);
   p.workgroups = (int)(units < most ? units : most);
   p.by_pair = pairs <= p.workgroups;
   return p;
