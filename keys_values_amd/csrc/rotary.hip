@@ -12,72 +12,119 @@ constexpr int NT = 256;
 
 template <int LPR>
 __device__ __forceinline__ float sum_over_row(float v) {
-#pragma unroll
-  for (int off = 1; off < LPR; off <<= 1) v += __shfl_xor(v, off, 64);
+  auto add = [](float x, auto ctrl) {
+    return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  v = add(v, std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
+  v = add(v, std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
+  v = add(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
+  if constexpr (LPR >= 16) v = add(v, std::integral_constant<int, 0x140>{});  // row_mirror
+  if constexpr (LPR == 32) {
+    const u32pair_t r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);  // the other row of the pair
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
   return v;
 }
 
-// A workgroup a token; LPR = D / 8 lanes a head, which hold 8 values each: pairs never leave a lane. Interleaved pairs lie side by side, and a lane holds a stretch of 8;
-// pairs of halves: four values of either half of the rotated part. Lanes behind that part hold stretches.
-template <int D, bool F16, bool INTERLEAVED>
-__global__ __launch_bounds__(NT) void rotary_kernel(const kvx_rotary_args a, const float factor) {
+// A workgroup a token, or several (grid y); LPR = D / 8 lanes a head, which hold 8 values each: pairs never leave a lane. Interleaved pairs lie side by side, and a lane
+// holds a stretch of 8; pairs of halves: four values of either half of the rotated part. Lanes behind that part hold stretches. `rows` heads of a workgroup at a
+// time, U of them a lane, every `stride` heads; a lane's angles and weights are the same for all of them.
+template <int D, bool F16, bool INTERLEAVED, int U>
+__global__ __launch_bounds__(512) void rotary_kernel(const kvx_rotary_args a, const float factor, const int rows, const int stride) {
   constexpr int LPR = D / 8;
   const int t = blockIdx.x, pos = a.positions[t];
-  if (pos < 0 || pos >= a.table_rows) return;
-  const int col = threadIdx.x % LPR, heads = a.Hq + a.Hkv, half = a.rotary_dim / 2;
+  const int col = threadIdx.x % LPR, mine = threadIdx.x / LPR, heads = a.Hq + a.Hkv, half = a.rotary_dim / 2;
   const bool turns = 8 * col < a.rotary_dim, split = !INTERLEAVED && turns;
   const int lo = split ? 4 * col : 8 * col, hi = split ? half + 4 * col : lo + 4;
+  uint16_t* token = (uint16_t*)a.qkv + t * a.stride_t;
+  u32x2_t x0[U], x1[U];
+  auto load = [&](int begin) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const uint16_t* p = token + min(begin + i * rows + mine, heads - 1) * D;
+      x0[i] = *(const u32x2_t*)(p + lo);
+      x1[i] = *(const u32x2_t*)(p + hi);
+    }
+  };
+  int begin = blockIdx.y * U * rows;
+  load(begin);  // does not wait for the position
+  if (pos < 0 || pos >= a.table_rows) return;
   f32x4_t cv = {1.0f, 1.0f, 1.0f, 1.0f}, sv = {0.0f, 0.0f, 0.0f, 0.0f};
   if (turns) {
     cv = *(const f32x4_t*)(a.cos + (int64_t)pos * half + 4 * col);
     sv = *(const f32x4_t*)(a.sin + (int64_t)pos * half + 4 * col);
   }
-  uint16_t* token = (uint16_t*)a.qkv + t * a.stride_t;
-  for (int first = 0; first < heads; first += NT / LPR) {  // all lanes stay: heads are reduced across them
-    const int head = first + (int)threadIdx.x / LPR, h = min(head, heads - 1);
-    uint16_t* p = token + h * D;
-    const u32x2_t x0 = *(const u32x2_t*)(p + lo), x1 = *(const u32x2_t*)(p + hi);
-    float y[8] = {elem_lo<F16>(x0[0]), elem_hi<F16>(x0[0]), elem_lo<F16>(x0[1]), elem_hi<F16>(x0[1]),
-                  elem_lo<F16>(x1[0]), elem_hi<F16>(x1[0]), elem_lo<F16>(x1[1]), elem_hi<F16>(x1[1])};
-    if (a.q_weight) {
-      float ss = 0.0f;
+  for (;;) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
-      const float n = sqrtf(sum_over_row<LPR>(ss)) * factor + a.eps;
-      const float* w = h < a.Hq ? a.q_weight : a.k_weight;
-      const f32x4_t w0 = *(const f32x4_t*)(w + lo), w1 = *(const f32x4_t*)(w + hi);
+    for (int i = 0; i < U; ++i) {
+      const int head = begin + i * rows + mine;
+      float y[8] = {elem_lo<F16>(x0[i][0]), elem_hi<F16>(x0[i][0]), elem_lo<F16>(x0[i][1]), elem_hi<F16>(x0[i][1]),
+                    elem_lo<F16>(x1[i][0]), elem_hi<F16>(x1[i][0]), elem_lo<F16>(x1[i][1]), elem_hi<F16>(x1[i][1])};
+      if (a.q_weight) {  // uniform
+        float ss = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = y[e] / n * (e < 4 ? w0[e] : w1[e - 4]);
+        for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
+        const float n = sqrtf(sum_over_row<LPR>(ss)) * factor + a.eps;
+        const float* w = head < a.Hq ? a.q_weight : a.k_weight;
+        const f32x4_t w0 = *(const f32x4_t*)(w + lo), w1 = *(const f32x4_t*)(w + hi);
+        const float inv = 1.0f / n;
+        if (__all(n > 0x1p-120f)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * (e < 4 ? w0[e] : w1[e - 4]);
+        } else {  // whose inverse is infinite, or NaN
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = y[e] / n * (e < 4 ? w0[e] : w1[e - 4]);
+        }
+      }
+      float z[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = INTERLEAVED ? 2 * e : e, k = INTERLEAVED ? 2 * e + 1 : e + 4;
+        z[j] = turns ? y[j] * cv[e] - y[k] * sv[e] : y[j];
+        z[k] = turns ? y[k] * cv[e] + y[j] * sv[e] : y[k];
+      }
+      if (head < heads) {
+        uint16_t* p = token + head * D;
+        *(u32x2_t*)(p + lo) = u32x2_t{pack_pair<F16>(z[0], z[1]), pack_pair<F16>(z[2], z[3])};
+        *(u32x2_t*)(p + hi) = u32x2_t{pack_pair<F16>(z[4], z[5]), pack_pair<F16>(z[6], z[7])};
+      }
     }
-    float z[8];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = INTERLEAVED ? 2 * e : e, j = INTERLEAVED ? 2 * e + 1 : e + 4;
-      z[i] = y[i] * cv[e] - y[j] * sv[e];
-      z[j] = y[j] * cv[e] + y[i] * sv[e];
-    }
-    if (!turns)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = y[e];
-    if (head < heads) {
-      *(u32x2_t*)(p + lo) = u32x2_t{pack_pair<F16>(z[0], z[1]), pack_pair<F16>(z[2], z[3])};
-      *(u32x2_t*)(p + hi) = u32x2_t{pack_pair<F16>(z[4], z[5]), pack_pair<F16>(z[6], z[7])};
-    }
+    begin += stride;
+    if (begin >= heads) break;
+    load(begin);
   }
 }
 
 template <int D>
 void launch_head(const kvx_rotary_args& a, hipStream_t st) {
   const float factor = 1.0f / sqrtf((float)D);
-  auto go = [&](auto f16, auto interleaved) {
-    hipLaunchKernelGGL((rotary_kernel<D, decltype(f16)::value, decltype(interleaved)::value>), dim3((unsigned)a.tokens), dim3(NT), 0, st, a, factor);
-  };
-  if (a.elem_dtype == KVX_KV_F16) {
-    if (a.interleaved) go(std::true_type{}, std::true_type{});
-    else go(std::true_type{}, std::false_type{});
-  } else {
-    if (a.interleaved) go(std::false_type{}, std::true_type{});
-    else go(std::false_type{}, std::false_type{});
+  constexpr int LPR = D / 8;
+  const int64_t lanes = (int64_t)(a.Hq + a.Hkv) * LPR;
+  // A token's heads over several workgroups where few tokens leave units idle or its heads are many; over one, two heads a lane, where up to 640 lanes of many
+  // tokens would read the angles again.
+  const int parts = lanes > 2 * NT + 128 || a.tokens <= 2 * num_cus() ? (int)min((lanes + NT - 1) / NT, (int64_t)65535) : 1;
+  const int each = parts > 1 || lanes <= NT ? 1 : 2;
+  const int threads = parts > 1 ? NT : (int)(lanes / each + 63) / 64 * 64, rows = threads / LPR;
+  const int64_t at_once = (1ll << 32) / threads / parts - 1;  // tokens whose threads a grid can count
+  for (int64_t done = 0; done < a.tokens; done += at_once) {
+    kvx_rotary_args part = a;
+    part.qkv = (uint16_t*)a.qkv + done * a.stride_t;
+    part.positions = a.positions + done;
+    const dim3 grid((unsigned)min(at_once, a.tokens - done), (unsigned)parts);
+    auto go = [&](auto f16, auto interleaved, auto u) {
+      hipLaunchKernelGGL((rotary_kernel<D, decltype(f16)::value, decltype(interleaved)::value, decltype(u)::value>), grid, dim3(threads), 0, st, part, factor, rows,
+                         parts * each * rows);
+    };
+    auto go_u = [&](auto f16, auto interleaved) {
+      if (each == 1) go(f16, interleaved, std::integral_constant<int, 1>{});
+      else go(f16, interleaved, std::integral_constant<int, 2>{});
+    };
+    auto go_layout = [&](auto f16) {
+      if (a.interleaved) go_u(f16, std::true_type{});
+      else go_u(f16, std::false_type{});
+    };
+    if (a.elem_dtype == KVX_KV_F16) go_layout(std::true_type{});
+    else go_layout(std::false_type{});
   }
 }
 
