@@ -29,7 +29,7 @@ __device__ __forceinline__ float sum_over_row(float v) {
 // A workgroup a token, or several (grid y); LPR = D / 8 lanes a head, which hold 8 values each: pairs never leave a lane. Interleaved pairs lie side by side, and a lane
 // holds a stretch of 8; pairs of halves: four values of either half of the rotated part. Lanes behind that part hold stretches. `rows` heads of a workgroup at a
 // time, U of them a lane, every `stride` heads; a lane's angles and weights are the same for all of them.
-template <int D, bool F16, bool INTERLEAVED, int U>
+template <int D, bool F16, bool INTERLEAVED, int U, bool PAST>  // PAST: loads and stores past the caches
 __global__ __launch_bounds__(512) void rotary_kernel(const kvx_rotary_args a, const float factor, const int rows, const int stride) {
   constexpr int LPR = D / 8;
   const int t = blockIdx.x, pos = a.positions[t];
@@ -37,13 +37,21 @@ __global__ __launch_bounds__(512) void rotary_kernel(const kvx_rotary_args a, co
   const bool turns = 8 * col < a.rotary_dim, split = !INTERLEAVED && turns;
   const int lo = split ? 4 * col : 8 * col, hi = split ? half + 4 * col : lo + 4;
   uint16_t* token = (uint16_t*)a.qkv + t * a.stride_t;
+  auto get = [](const u32x2_t* p) {
+    if constexpr (PAST) return __builtin_nontemporal_load(p);
+    else return *p;
+  };
+  auto put = [](u32x2_t v, u32x2_t* p) {
+    if constexpr (PAST) __builtin_nontemporal_store(v, p);
+    else *p = v;
+  };
   u32x2_t x0[U], x1[U];
   auto load = [&](int begin) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const uint16_t* p = token + min(begin + i * rows + mine, heads - 1) * D;
-      x0[i] = *(const u32x2_t*)(p + lo);
-      x1[i] = *(const u32x2_t*)(p + hi);
+      x0[i] = get((const u32x2_t*)(p + lo));
+      x1[i] = get((const u32x2_t*)(p + hi));
     }
   };
   int begin = blockIdx.y * U * rows;
@@ -85,8 +93,8 @@ __global__ __launch_bounds__(512) void rotary_kernel(const kvx_rotary_args a, co
       }
       if (head < heads) {
         uint16_t* p = token + head * D;
-        *(u32x2_t*)(p + lo) = u32x2_t{pack_pair<F16>(z[0], z[1]), pack_pair<F16>(z[2], z[3])};
-        *(u32x2_t*)(p + hi) = u32x2_t{pack_pair<F16>(z[4], z[5]), pack_pair<F16>(z[6], z[7])};
+        put(u32x2_t{pack_pair<F16>(z[0], z[1]), pack_pair<F16>(z[2], z[3])}, (u32x2_t*)(p + lo));
+        put(u32x2_t{pack_pair<F16>(z[4], z[5]), pack_pair<F16>(z[6], z[7])}, (u32x2_t*)(p + hi));
       }
     }
     begin += stride;
@@ -105,6 +113,10 @@ void launch_head(const kvx_rotary_args& a, hipStream_t st) {
   const int parts = lanes > 2 * NT + 128 || a.tokens <= 2 * num_cus() ? (int)min((lanes + NT - 1) / NT, (int64_t)65535) : 1;
   const int each = parts > 1 || lanes <= NT ? 1 : 2;
   const int threads = parts > 1 ? NT : (int)(lanes / each + 63) / 64 * 64, rows = threads / LPR;
+  // More than 64 MB goes past the caches; less was just written and may be found in the one that the dies share. us, through / past them: 16384 tokens of 40 heads of 128
+  // 69.0 / 63.4 (5.4 TB/s), of 32 heads of 128, half of each, 51.8 / 44.8; 4096 of 40, read from memory, 22.2 / 19.0, but 5001 of 32 in turn with two other batches
+  // 13.7 / 15.4, 16384 of 10 heads of 64, 21 MB, 10.0 / 11.0.
+  const bool past = a.tokens * (a.Hq + a.Hkv) * D * 2 > (64ll << 20);
   const int64_t at_once = (1ll << 32) / threads / parts - 1;  // tokens whose threads a grid can count
   for (int64_t done = 0; done < a.tokens; done += at_once) {
     kvx_rotary_args part = a;
@@ -112,8 +124,10 @@ void launch_head(const kvx_rotary_args& a, hipStream_t st) {
     part.positions = a.positions + done;
     const dim3 grid((unsigned)min(at_once, a.tokens - done), (unsigned)parts);
     auto go = [&](auto f16, auto interleaved, auto u) {
-      hipLaunchKernelGGL((rotary_kernel<D, decltype(f16)::value, decltype(interleaved)::value, decltype(u)::value>), grid, dim3(threads), 0, st, part, factor, rows,
-                         parts * each * rows);
+      constexpr bool F16 = decltype(f16)::value, IL = decltype(interleaved)::value;
+      constexpr int U = decltype(u)::value;
+      if (past) hipLaunchKernelGGL((rotary_kernel<D, F16, IL, U, true>), grid, dim3(threads), 0, st, part, factor, rows, parts * each * rows);
+      else hipLaunchKernelGGL((rotary_kernel<D, F16, IL, U, false>), grid, dim3(threads), 0, st, part, factor, rows, parts * each * rows);
     };
     auto go_u = [&](auto f16, auto interleaved) {
       if (each == 1) go(f16, interleaved, std::integral_constant<int, 1>{});
