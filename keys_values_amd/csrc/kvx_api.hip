@@ -516,9 +516,12 @@ static int check_pages(const kvx_pages& p, const char* who) {
   // a page's rows are addressed from its first by 32-bit byte offsets
   KVX_REQUIRE(p.k_stride_t >= row && p.v_stride_t >= row && p.k_stride_t <= (1 << 19) && p.v_stride_t <= (1 << 19), KVX_ERR_UNSUPPORTED,
               "%s: slot strides %lld, %lld outside [%d, 2^19]", who, (long long)p.k_stride_t, (long long)p.v_stride_t, row);
-  // pages are addressed by products of 32 bits
-  KVX_REQUIRE(p.k_stride_page < ((int64_t)1 << 31) && p.v_stride_page < ((int64_t)1 << 31) && (plain || p.qs_stride_page < ((int64_t)1 << 30)), KVX_ERR_UNSUPPORTED,
-              "%s: page strides %lld, %lld beyond 2^31", who, (long long)p.k_stride_page, (long long)p.v_stride_page);
+  // pages and heads are addressed by products of 32 bits
+  constexpr int64_t kMost = (int64_t)1 << 31;
+  KVX_REQUIRE(p.k_stride_page < kMost && p.v_stride_page < kMost && p.k_stride_h < kMost && p.v_stride_h < kMost &&
+                  (plain || (p.qs_stride_page < kMost / 2 && p.qs_stride_h < kMost / 2)),
+              KVX_ERR_UNSUPPORTED, "%s: page strides %lld, %lld or head strides %lld, %lld beyond 2^31", who, (long long)p.k_stride_page, (long long)p.v_stride_page,
+              (long long)p.k_stride_h, (long long)p.v_stride_h);
   if (!plain) {
     KVX_REQUIRE(p.k_scale && p.k_zp && p.v_scale && p.v_zp, KVX_ERR_INVALID, "%s: pages of codes need scales and zero points", who);
     KVX_REQUIRE(aligned16(p.k_scale) && aligned16(p.k_zp) && aligned16(p.v_scale) && aligned16(p.v_zp) && p.qs_stride_page >= 0 && p.qs_stride_h >= 0 &&

@@ -30,20 +30,28 @@ constexpr int NT = 256, WAVES = 4, UNIT = 128;  // keys of a step: a block of 32
 constexpr float kLowest = -3.4028235e38f;       // running maximum before the first key
 typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 
+// The first line is read first: what a workgroup's share follows from.
 struct PagedParams {
-  kvx_paged_decode_args a;
-  float c;          // sm_scale * log2(e)
-  int shift;        // log2 of the page size
-  int cap;          // tokens of a table's pages
-  int Gr;           // query heads per KV head
-  int workgroups;
-  int cus;          // compute units
-  int unit;         // log2 of the keys of a unit
-  uint32_t k_page, v_page, q_page;  // bytes from page to page of K, V and the quantiser's arrays
-  int by_pair;      // part_of goes by pairs, which are fewer, else by workgroups
-  float* part_o;    // (2 workgroups, Gr, D)
-  float* part_ml;   // (2 workgroups, Gr, 2): maximum and sum
-  int* part_of;     // by pairs: the workgroup that left a pair's first partial; by workgroups: the pair; and how many partials the pair has, 0: none
+  const int* lens;
+  const int* table;
+  int64_t table_sb;
+  int B, Hkv, cap /* tokens of a table's pages */, unit /* log2 of the keys of a unit */, cus /* compute units */, workgroups, shift /* log2 of the page size */, max_pages;
+  int num_pages, Gr /* query heads per KV head */;
+
+  const uint16_t* q;
+  int64_t q_sb, q_sh;
+  const uint8_t *k, *v;
+  const uint32_t *k_scale, *k_zp, *v_scale, *v_zp;
+  uint32_t k_page, v_page, q_page, k_head, v_head, q_head, k_row, v_row;  // bytes from page to page, head to head, row to row of K, V and the quantiser's arrays
+  float c;      // sm_scale * log2(e)
+  int by_pair;  // part_of goes by pairs, which are fewer, else by workgroups
+
+  uint16_t* o;
+  int64_t o_sb, o_sh;
+  float* lse;      // or NULL
+  float* part_o;   // (2 workgroups, Gr, D)
+  float* part_ml;  // (2 workgroups, Gr, 2): maximum and sum
+  int* part_of;    // by pairs: the workgroup that left a pair's first partial; by workgroups: the pair; and how many partials the pair has, 0: none. NULL: no partials
 };
 
 __device__ __forceinline__ int units_of(int len, int cap, int unit) { return max(1, (min(max(len, 0), cap) + (1 << unit) - 1) >> unit); }
@@ -170,8 +178,9 @@ __device__ __forceinline__ float sum_groups(float x) {
 template <typename T>
 __device__ __forceinline__ T once(const void* p) { return __builtin_nontemporal_load((const T*)p); }
 
-// Wavefronts a SIMD that the registers have to leave room for: plain rows of 256 values take more than half of them.
-constexpr int waves_per_simd(int D, bool codes) { return D == 256 && !codes ? 1 : 2; }
+// Wavefronts a SIMD that the registers have to leave room for. Plain rows of 256 values take more than half of them. Plain rows of 128 fit a third wavefront only if
+// asked to, which short pairs gain from (256 sequences of 50 to 400 tokens, 32 / 8 heads: 49.1 us with two, 42.8 with three). No bound here spills.
+constexpr int waves_per_simd(int D, bool codes) { return D == 256 && !codes ? 1 : D == 128 && !codes ? 3 : 2; }
 
 template <int D, int KV>
 __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged_decode_kernel(const PagedParams p) {
@@ -181,21 +190,20 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
   // The running maximum moves when a logit exceeds it by kTop. Weights in fp16 are kept below 2^15, and brought to 2^7 when it moves: what is a normal number
   // there goes down to 2^-21 of the largest then, and what is not zero to 2^-32.
   constexpr float kTop = P16 ? 15.0f : 8.0f, kBias = P16 ? 7.0f : 0.0f;
-  // The part of a weight that its 16 bits drop is a second operand where outputs have as many bits: the rounding of weights would be as large as theirs.
-  constexpr bool FINE = F16;
+  // The part of a weight that its 16 bits drop is a second operand where outputs have as many bits: the rounding of weights would be as large as theirs. It is not
+  // seen in the time (16 sequences of 16384, plain rows of 128: 157.9 and 158.1 us).
+  constexpr bool FINE = F16 || !CODES;
   constexpr int RS = D + 4;  // floats of a head's row in LDS: heads in different banks
   __shared__ __align__(16) float red[WAVES][16][RS];
   __shared__ __align__(16) float state[WAVES][2][64];
   __shared__ float red_m[WAVES][16], red_l[WAVES][16];
 
-  const kvx_pages& pg = p.a.pages;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, kg = lane >> 4;
-  const int B = p.a.B, Hkv = pg.Hkv, w = blockIdx.x, mask = pg.page_size - 1;
-  const int* const lens = p.a.lens;
+  const int B = p.B, Hkv = p.Hkv, w = blockIdx.x, mask = (1 << p.shift) - 1;
 
   // ---- this workgroup's units: every wavefront finds them for itself, 64 sequences at a time
   const int windows = (B + 63) / 64;
-  auto window = [&](int i) { return 64 * i + lane < B ? lens[64 * i + lane] : -1; };
+  auto window = [&](int i) { return 64 * i + lane < B ? p.lens[64 * i + lane] : -1; };
   auto units_in = [&](int len, int i) { return 64 * i + lane < B ? units_of(len, p.cap, p.unit) : 0; };
   int lane_len = 0, mine = 0;  // lane_len: of sequence (b & ~63) + lane
   for (int i = 0; i < windows; ++i) {
@@ -208,7 +216,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
   // one, whose partials are the fewest, where pairs are long and rows of 128 bytes and more keep enough of them on their way (16 x 16384, plain rows of 128: 158.3, 162.0
   // with two, 165.6 with three; but 4-bit rows of 128: 65.7, 53.7 with two).
   constexpr bool WIDE = D * ES >= (U4 ? 256 : 128);
-  const int pairs = B * Hkv, sharing = total <= 4 * pairs ? p.workgroups : WIDE && total >= 64 * pairs ? p.cus : 2 * p.cus;
+  const int pairs = B * Hkv, sharing = (total + 3) / 4 <= pairs ? p.workgroups : WIDE && total / 64 >= pairs ? p.cus : 2 * p.cus;
   const Shares shares(total, min(sharing, p.workgroups));
   int unit = shares.first(w);  // the next unit
   const int end = shares.first(w + 1);
@@ -253,8 +261,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
     return s;
   };
 
-  const uint32_t k_rowb = (uint32_t)pg.k_stride_t * ES, v_rowb = (uint32_t)pg.v_stride_t * ES;
-  const uint32_t k_lane = (uint32_t)m * k_rowb + (U4 && D == 64 ? 8 : 16) * kg, v_lane = 4 * kg * v_rowb + (uint32_t)m * R::VB;
+  const uint32_t k_lane = (uint32_t)m * p.k_row + (U4 && D == 64 ? 8 : 16) * kg, v_lane = 4 * kg * p.v_row + (uint32_t)m * R::VB;
 
   // ---- rows of a block of 32 keys. Lane 2 j + gi holds the page of half gi of the wavefront's block j (of 32 at a time). A page that the pool does not have is
   // read as page 0, and its keys are masked behind. Keys behind the end lie in the same pages, or masked ones.
@@ -275,7 +282,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
   const uint8_t *k_head, *v_head;
   const char *k_state, *v_state;
   auto pages_of = [&](const Stretch& s, int j) {
-    return p.a.block_table[s.b * p.a.bt_stride_b + min((s.k_begin + 32 * wave + (j + (lane >> 1)) * UNIT + 16 * (lane & 1)) >> p.shift, p.a.max_pages - 1)];
+    return p.table[s.b * p.table_sb + min((s.k_begin + 32 * wave + (j + (lane >> 1)) * UNIT + 16 * (lane & 1)) >> p.shift, p.max_pages - 1)];
   };
   auto tiles = [&](int j) {
     if (j > 0 && (j & 31) == 0) {
@@ -284,8 +291,8 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
     }
     Tiles t;
     const int page0 = __builtin_amdgcn_readlane(lane_page, 2 * (j & 31)), page1 = __builtin_amdgcn_readlane(lane_page, 2 * (j & 31) + 1);
-    t.ok0 = (uint32_t)page0 < (uint32_t)pg.num_pages;
-    t.ok1 = (uint32_t)page1 < (uint32_t)pg.num_pages;
+    t.ok0 = (uint32_t)page0 < (uint32_t)p.num_pages;
+    t.ok1 = (uint32_t)page1 < (uint32_t)p.num_pages;
     t.page0 = t.ok0 ? page0 : 0;
     t.page1 = t.ok1 ? page1 : 0;
     return t;
@@ -298,7 +305,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
 #pragma unroll
     for (int gi = 0; gi < 2; ++gi) {
       const uint8_t* base = k_head + (uint64_t)(uint32_t)t.page(gi) * p.k_page;
-      const uint32_t off = (uint32_t)((chunk + 16 * gi) & mask) * k_rowb + k_lane;
+      const uint32_t off = (uint32_t)((chunk + 16 * gi) & mask) * p.k_row + k_lane;
 #pragma unroll
       for (int x = 0; x < R::KR; ++x) {
         if constexpr (U4 && D == 64) {
@@ -316,10 +323,10 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
 #pragma unroll
     for (int gi = 0; gi < 2; ++gi) {
       const uint8_t* base = v_head + (uint64_t)(uint32_t)t.page(gi) * p.v_page;
-      const uint32_t off = (uint32_t)((chunk + 16 * gi) & mask) * v_rowb + v_lane;
+      const uint32_t off = (uint32_t)((chunk + 16 * gi) & mask) * p.v_row + v_lane;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint8_t* row = base + (off + (uint32_t)i * v_rowb);
+        const uint8_t* row = base + (off + (uint32_t)i * p.v_row);
         uint32_t(&x)[R::VW] = r.w[4 * gi + i];
         if constexpr (R::VB >= 16) {
 #pragma unroll
@@ -338,9 +345,9 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
       }
     }
   };
-  // Queries, B operands of the first product: head m (zero beyond the group)
+  // Queries, B operands of the first product: head m
   auto load_q = [&](u32x4_t (&q)[KJ], const Stretch& s) {
-    const uint16_t* row = (const uint16_t*)p.a.q + s.b * p.a.q_stride_b + (int64_t)(s.h * p.Gr + min(m, p.Gr - 1)) * p.a.q_stride_h;
+    const uint16_t* row = p.q + s.b * p.q_sb + (int64_t)(s.h * p.Gr + min(m, p.Gr - 1)) * p.q_sh;
 #pragma unroll
     for (int e = 0; e < KJ; ++e) q[e] = *(const u32x4_t*)(row + R::kslice(e, kg));
   };
@@ -351,12 +358,12 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
   auto start = [&](const Stretch& s, int page) {
     at = s;
     lane_page = page;
-    k_head = (const uint8_t*)pg.k + s.h * pg.k_stride_h * ES;
-    v_head = (const uint8_t*)pg.v + s.h * pg.v_stride_h * ES;
+    k_head = p.k + (uint64_t)(uint32_t)s.h * p.k_head;
+    v_head = p.v + (uint64_t)(uint32_t)s.h * p.v_head;
     if constexpr (CODES) {
-      const int64_t q = s.h * pg.qs_stride_h + m;
-      k_state = (const char*)((lane < 32 ? (const uint32_t*)pg.k_scale : (const uint32_t*)pg.k_zp) + q);
-      v_state = (const char*)((lane < 32 ? (const uint32_t*)pg.v_scale : (const uint32_t*)pg.v_zp) + q);
+      const uint64_t q = (uint64_t)(uint32_t)s.h * p.q_head + 4 * m;
+      k_state = (const char*)(lane < 32 ? p.k_scale : p.k_zp) + q;
+      v_state = (const char*)(lane < 32 ? p.v_scale : p.v_zp) + q;
     }
     t = tiles(0);
     load_q(qb, s);
@@ -382,6 +389,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
     }
 
     float qsum = 0.0f, to_logit = p.c;
+    // Columns beyond the group are zeros: with copies of the last head there the matrix cores are slower (16 x 16384, 32 / 8 heads of 64, plain: 84.5 us, 90.5)
 #pragma unroll
     for (int e = 0; e < KJ; ++e)
       if (m >= p.Gr) qb[e] = u32x4_t{0u, 0u, 0u, 0u};
@@ -609,9 +617,8 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
       for (int j = 0; j < WAVES; ++j) x += *(const f32x4_t*)&red[j][g][d] * f[j];
       if (alone) {
         x *= sum == 0.0f ? 0.0f : 1.0f / sum;
-        *(u32x2_t*)((uint16_t*)p.a.o + now.b * p.a.o_stride_b + (int64_t)(now.h * p.Gr + g) * p.a.o_stride_h + d) =
-            u32x2_t{pack_pair<F16>(x[0], x[1]), pack_pair<F16>(x[2], x[3])};
-        if (d == 0 && p.a.lse) p.a.lse[(int64_t)now.b * p.a.Hq + now.h * p.Gr + g] = sum == 0.0f ? -INFINITY : top + fast_log2(sum);
+        *(u32x2_t*)(p.o + now.b * p.o_sb + (int64_t)(now.h * p.Gr + g) * p.o_sh + d) = u32x2_t{pack_pair<F16>(x[0], x[1]), pack_pair<F16>(x[2], x[3])};
+        if (d == 0 && p.lse) p.lse[((int64_t)now.b * Hkv + now.h) * p.Gr + g] = sum == 0.0f ? -INFINITY : top + fast_log2(sum);
       } else {
         *(f32x4_t*)(p.part_o + ((int64_t)slot * p.Gr + g) * D + d) = x;
         if (d == 0) *(f32x2_t*)(p.part_ml + ((int64_t)slot * p.Gr + g) * 2) = f32x2_t{top, sum};
@@ -635,7 +642,7 @@ __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedParams p) {
   __shared__ __align__(16) float red[GROUPS][LANES][4];
   __shared__ float red_m[GROUPS][LANES], red_l[GROUPS][LANES];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES, i = blockIdx.y * 4 * LANES + 4 * lane, g = min(i / D, p.Gr - 1), d = i % D;
-  const int w = p.by_pair ? at : blockIdx.x, pair = p.by_pair ? blockIdx.x : at, b = pair / p.a.pages.Hkv, h = pair - b * p.a.pages.Hkv;
+  const int w = p.by_pair ? at : blockIdx.x, pair = p.by_pair ? blockIdx.x : at, b = pair / p.Hkv, h = pair - b * p.Hkv;
   float top = kLowest, sum = 0.0f;
   f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int s0 = group; s0 < n; s0 += GROUPS * U) {
@@ -680,38 +687,65 @@ __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedParams p) {
     x += *(const f32x4_t*)red[j][lane] * f;
   }
   x *= sum == 0.0f ? 0.0f : 1.0f / sum;
-  *(u32x2_t*)((uint16_t*)p.a.o + b * p.a.o_stride_b + (int64_t)(h * p.Gr + g) * p.a.o_stride_h + d) = u32x2_t{pack_pair<F16>(x[0], x[1]), pack_pair<F16>(x[2], x[3])};
-  if (p.a.lse && d == 0) p.a.lse[(int64_t)b * p.a.Hq + h * p.Gr + g] = sum == 0.0f ? -INFINITY : all + fast_log2(sum);
+  *(u32x2_t*)(p.o + b * p.o_sb + (int64_t)(h * p.Gr + g) * p.o_sh + d) = u32x2_t{pack_pair<F16>(x[0], x[1]), pack_pair<F16>(x[2], x[3])};
+  if (p.lse && d == 0) p.lse[(int64_t)pair * p.Gr + g] = sum == 0.0f ? -INFINITY : all + fast_log2(sum);
 }
 
 PagedParams params_of(const kvx_paged_decode_args& a) {
+  const kvx_pages& g = a.pages;
+  const bool plain = kv_is_plain(g.kv_dtype);
+  const int es = plain ? 2 : 1;
   PagedParams p{};
-  p.a = a;
-  p.c = a.sm_scale * kLog2e;
-  p.shift = __builtin_ctz(a.pages.page_size);
-  const int es = kv_is_plain(a.pages.kv_dtype) ? 2 : 1;
-  p.k_page = (uint32_t)(a.pages.k_stride_page * es);
-  p.v_page = (uint32_t)(a.pages.v_stride_page * es);
-  p.q_page = (uint32_t)(a.pages.qs_stride_page * 4);
+  p.lens = a.lens;
+  p.table = a.block_table;
+  p.table_sb = a.bt_stride_b;
+  p.B = a.B;
+  p.Hkv = g.Hkv;
+  p.shift = __builtin_ctz(g.page_size);
+  p.max_pages = a.max_pages;
   p.cap = a.max_pages << p.shift;
-  p.Gr = a.Hq / a.pages.Hkv;
+  p.num_pages = g.num_pages;
+  p.Gr = a.Hq / g.Hkv;
+  p.q = (const uint16_t*)a.q;
+  p.q_sb = a.q_stride_b;
+  p.q_sh = a.q_stride_h;
+  p.k = (const uint8_t*)g.k;
+  p.v = (const uint8_t*)g.v;
+  p.k_scale = (const uint32_t*)g.k_scale;
+  p.k_zp = (const uint32_t*)g.k_zp;
+  p.v_scale = (const uint32_t*)g.v_scale;
+  p.v_zp = (const uint32_t*)g.v_zp;
+  p.k_page = (uint32_t)(g.k_stride_page * es);
+  p.v_page = (uint32_t)(g.v_stride_page * es);
+  p.k_head = (uint32_t)(g.k_stride_h * es);
+  p.v_head = (uint32_t)(g.v_stride_h * es);
+  p.k_row = (uint32_t)(g.k_stride_t * es);
+  p.v_row = (uint32_t)(g.v_stride_t * es);
+  if (!plain) {
+    p.q_page = (uint32_t)(g.qs_stride_page * 4);
+    p.q_head = (uint32_t)(g.qs_stride_h * 4);
+  }
+  p.c = a.sm_scale * kLog2e;
+  p.o = (uint16_t*)a.o;
+  p.o_sb = a.o_stride_b;
+  p.o_sh = a.o_stride_h;
+  p.lse = a.lse;
   // Tables of up to 512 tokens: a pair is a workgroup's, and there is no second launch.
   p.unit = p.cap <= 4 * UNIT ? 9 : 7;
   p.cus = num_cus();
   // One workgroup a compute unit for the only pair: the partials of more take longer to join than they save (one of 100000 tokens, 16 heads of 128: 21.7 us, 33.8
   // with three).
-  const int64_t per_cu = a.pages.D == 256 ? waves_per_simd(256, !kv_is_plain(a.pages.kv_dtype)) : 3;
+  const int64_t per_cu = g.D == 256 ? waves_per_simd(256, !plain) : 3;
   const int64_t pairs = (int64_t)a.B * a.pages.Hkv, units = pairs * ((p.cap + (1 << p.unit) - 1) >> p.unit), most = p.cus * (pairs < per_cu ? pairs : per_cu);
   p.workgroups = (int)(units < most ? units : most);
   p.by_pair = pairs <= p.workgroups;
   return p;
 }
-int64_t pairs_of(const PagedParams& p) { return (int64_t)p.a.B * p.a.pages.Hkv; }
 bool splits(const PagedParams& p) { return p.cap > (1 << p.unit); }
 
 template <int D>
-void launch_head(const PagedParams& p, hipStream_t st) {
-  switch (p.a.pages.kv_dtype) {
+void launch_head(const PagedParams& p, int kv_dtype, hipStream_t st) {
+  switch (kv_dtype) {
 #define KVX_PAGES_CASE(KV) case KV: hipLaunchKernelGGL((paged_decode_kernel<D, KV>), dim3(p.workgroups), dim3(NT), 0, st, p); break;
     KVX_PAGES_CASE(KVX_KV_BF16)
     KVX_PAGES_CASE(KVX_KV_F16)
@@ -722,36 +756,36 @@ void launch_head(const PagedParams& p, hipStream_t st) {
 #undef KVX_PAGES_CASE
   }
   if (!splits(p)) return;
-  const unsigned rows = p.by_pair ? (unsigned)pairs_of(p) : (unsigned)p.workgroups;
+  const unsigned rows = p.by_pair ? (unsigned)(p.B * p.Hkv) : (unsigned)p.workgroups;
   auto join = [&](auto lanes) {
     constexpr int LANES = decltype(lanes)::value;
     const dim3 grid(rows, (p.Gr * D + 4 * LANES - 1) / (4 * LANES));
-    if (kv_elem_f16(p.a.pages.kv_dtype)) hipLaunchKernelGGL((paged_join_kernel<D, true, LANES>), grid, dim3(NT), 0, st, p);
+    if (kv_elem_f16(kv_dtype)) hipLaunchKernelGGL((paged_join_kernel<D, true, LANES>), grid, dim3(NT), 0, st, p);
     else hipLaunchKernelGGL((paged_join_kernel<D, false, LANES>), grid, dim3(NT), 0, st, p);
   };
   if (rows <= 64) join(std::integral_constant<int, 16>{});
   else join(std::integral_constant<int, 64>{});
 }
 
-size_t part_floats(const PagedParams& p) { return (size_t)2 * p.workgroups * p.Gr * p.a.pages.D; }
+size_t part_floats(const PagedParams& p, int D) { return (size_t)2 * p.workgroups * p.Gr * D; }
 
 }  // namespace
 
 size_t paged_decode_workspace(const kvx_paged_decode_args& a) {
   const PagedParams p = params_of(a);
-  return splits(p) ? 4 * (part_floats(p) + (size_t)4 * p.workgroups * p.Gr + 2 * p.workgroups) : 0;
+  return splits(p) ? 4 * (part_floats(p, a.pages.D) + (size_t)4 * p.workgroups * p.Gr + 2 * p.workgroups) : 0;
 }
 
 int launch_paged_decode(const kvx_paged_decode_args& a, hipStream_t st) {
   PagedParams p = params_of(a);
   if (splits(p)) {
     p.part_o = (float*)a.workspace;
-    p.part_ml = p.part_o + part_floats(p);
+    p.part_ml = p.part_o + part_floats(p, a.pages.D);
     p.part_of = (int*)(p.part_ml + (size_t)4 * p.workgroups * p.Gr);
   }
-  if (a.pages.D == 256) launch_head<256>(p, st);
-  else if (a.pages.D == 128) launch_head<128>(p, st);
-  else launch_head<64>(p, st);
+  if (a.pages.D == 256) launch_head<256>(p, a.pages.kv_dtype, st);
+  else if (a.pages.D == 128) launch_head<128>(p, a.pages.kv_dtype, st);
+  else launch_head<64>(p, a.pages.kv_dtype, st);
   KVX_HIP(hipGetLastError());
   return KVX_OK;
 }

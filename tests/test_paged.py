@@ -88,7 +88,7 @@ BAD_PAGES = [
     (dict(v_stride_page=-4096), "INVALID"), (dict(page_size=0), "UNSUPPORTED"), (dict(page_size=8), "UNSUPPORTED"), (dict(page_size=48), "UNSUPPORTED"),
     (dict(page_size=2048), "UNSUPPORTED"), (dict(D=96), "UNSUPPORTED"), (dict(kv_dtype=6), "UNSUPPORTED"), (dict(kv_dtype=-1), "UNSUPPORTED"),
     (dict(k_stride_t=64), "UNSUPPORTED"), (dict(v_stride_t=2**20), "UNSUPPORTED"), (dict(Hkv=65536), "UNSUPPORTED"),
-    (dict(k_stride_page=2**31), "UNSUPPORTED"), (dict(v_stride_page=2**40), "UNSUPPORTED"), (dict(kv_dtype=_lib.KVX_KV_U8, qs_stride_page=2**30), "UNSUPPORTED"),
+    (dict(k_stride_page=2**31), "UNSUPPORTED"), (dict(v_stride_page=2**40), "UNSUPPORTED"), (dict(k_stride_h=2**31), "UNSUPPORTED"), (dict(kv_dtype=_lib.KVX_KV_U8, qs_stride_page=2**30), "UNSUPPORTED"),
     (dict(kv_dtype=_lib.KVX_KV_U8, k_scale=0), "INVALID"), (dict(kv_dtype=_lib.KVX_KV_U8, v_zp=4100), "INVALID"),
     (dict(kv_dtype=_lib.KVX_KV_U8, qs_stride_h=18), "INVALID"), (dict(kv_dtype=_lib.KVX_KV_U8, k_stride_t=136), "INVALID"),
 ]
