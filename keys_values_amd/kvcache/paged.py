@@ -76,6 +76,10 @@ class PagedKVCacheBuffers:
     def slots(self, block_table: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """Slots of the tokens at ``positions`` (sequences, tokens) of the sequences of ``block_table``, flat int64; -1 for a negative position and
         for one behind the table. Once per step: the layers share them."""
+        if block_table.dim() != 2 or block_table.shape[1] == 0:
+            raise ValueError(f"block_table must be (sequences, pages), got shape {tuple(block_table.shape)}")
+        if positions.dim() != 2 or positions.shape[0] != block_table.shape[0]:
+            raise ValueError(f"positions must be ({block_table.shape[0]}, tokens), got shape {tuple(positions.shape)}")
         pos = positions.long()
         page = torch.div(pos.clamp(min=0), self.page_size, rounding_mode="floor")
         there = (pos >= 0) & (page < block_table.shape[1])

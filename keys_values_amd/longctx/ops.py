@@ -40,6 +40,8 @@ class RopeScaling:
             raise ValueError(f"low_freq_factor = {self.low_freq_factor} must be positive and below high_freq_factor = {self.high_freq_factor}")
         if self.kind == "yarn" and not (0.0 < self.beta_slow < self.beta_fast):
             raise ValueError(f"beta_slow = {self.beta_slow} must be positive and below beta_fast = {self.beta_fast}")
+        if self.kind == "yarn" and not (self.original_context > 2.0 * math.pi * self.beta_slow):  # the first pair turns original_context / 2 pi times
+            raise ValueError(f"original_context = {self.original_context}: no pair turns beta_slow = {self.beta_slow} times over it")
 
     def frequencies(self, rotary_dim: int, base: float) -> torch.Tensor:
         """Angle per position of pair j, float64 (rotary_dim / 2,)."""

@@ -4,6 +4,7 @@ import ctypes
 import math
 import os
 import subprocess
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -192,6 +193,24 @@ def test_pools_are_checked(error, kwargs):
         PagedKVCacheBuffers(**{**dict(num_pages=4, page_size=16, n_query_groups=2, head_size=64, device="cpu"), **kwargs})
     with pytest.raises(ValueError, match="head_size and dtype"):
         paged_read(None, None, None, None, 4, quant=())
+
+
+def test_slots_are_checked():
+    slots, pool = PagedKVCacheBuffers.slots, SimpleNamespace(page_size=16)
+    table = torch.tensor([[3, 1], [0, -1]], dtype=torch.int32)
+    assert slots(pool, table, torch.tensor([[0, 17], [-1, 16]])).tolist() == [48, 17, -1, -1]
+    assert slots(pool, table[:0], torch.empty(0, 5, dtype=torch.int32)).shape == (0,)
+    for bad, positions in ((table[:, :0], torch.zeros(2, 1)), (table[0], torch.zeros(2, 1)), (table, torch.zeros(1, 4)), (table, torch.zeros(3, 4)), (table, torch.zeros(2))):
+        with pytest.raises(ValueError):
+            slots(pool, bad, positions.int())
+
+
+def test_a_context_without_a_turn_is_refused():
+    rows.RopeScaling("yarn", 2.0, original_context=7)
+    rows.RopeScaling("linear", 2.0, original_context=1)
+    for kwargs in (dict(original_context=6), dict(original_context=60, beta_slow=10.0)):
+        with pytest.raises(ValueError):
+            rows.RopeScaling("yarn", 2.0, **kwargs)
 
 
 # ---- angles of long contexts ----------------------------------------------------------------------------------------
