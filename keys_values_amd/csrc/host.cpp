@@ -961,7 +961,8 @@ PyObject* rotary(PyObject* const* args, Py_ssize_t n) {
           shape_str(qkv).c_str());
   // the tokens' axes as one: in place, so a copy would not do
   int64_t tokens = 1, stride = 0;
-  for (int64_t i = qkv.dim() - 2; i >= 0; --i) {
+  if (qkv.numel() == 0) tokens = 0;
+  for (int64_t i = qkv.dim() - 2; i >= 0 && tokens > 0; --i) {
     if (qkv.size(i) == 1) continue;
     if (tokens == 1) stride = qkv.stride(i);
     else if (qkv.stride(i) != stride * tokens) raise(PyExc_ValueError, "the tokens of qkv must lie at one stride");

@@ -504,7 +504,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
         constexpr float MID = U4 ? 8.0f : 128.0f;
         float mine = lane < 32 ? __uint_as_float(v.state) : (float)(int32_t)v.state - MID;
         if (masked && !live(chunk, (lane >> 4) & 1, m)) mine = 0.0f;
-        const float scale = lane < 32 ? mine : 0.0f;
+        const float scale = lane < 32 ? fabsf(mine) : 0.0f;
         if (__any(scale > unit_v)) {
           const int ex = min((int)(__float_as_uint(max_lanes(scale)) >> 23) + 1, 253);
           const float per = __uint_as_float((uint32_t)(254 - ex) << 23), al = unit_v * per;

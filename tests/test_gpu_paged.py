@@ -163,6 +163,65 @@ def test_decode_of_batches(gpu, store, B, Hq, Hkv, D, page, low, high):
     decode_and_check(pool, gpu, Hq)
 
 
+@pytest.mark.parametrize("store,B,Hq,Hkv,D,low,high", [
+    ("bf16", 500, 2, 2, 64, 0, 150),    # more pairs than workgroups
+    ("u4", 260, 8, 4, 64, 1, 100),
+    ("fp16", 130, 7, 7, 128, 1, 9),
+    ("u8", 300, 3, 3, 256, 0, 60),
+])
+def test_decode_of_more_pairs_than_workgroups(gpu, store, B, Hq, Hkv, D, low, high):
+    gen = torch.Generator().manual_seed(B)
+    lens = torch.randint(low, high + 1, (B,), generator=gen).tolist()
+    lens[B // 2], lens[-1] = 3000, 700
+    pool = Pool(gpu, store, lens, Hkv, D, 32, seed=B)
+    decode_and_check(pool, gpu, Hq)
+
+
+@pytest.mark.parametrize("store", STORES)
+@pytest.mark.parametrize("page,width", [(16, 32), (512, 1), (16, 33), (128, 4), (1024, 1)])
+def test_decode_of_tables_around_512_tokens(gpu, store, page, width):
+    """Up to 512 tokens, nothing is joined."""
+    lens = [512, 511, 1, 0, 385, 129]
+    pool = Pool(gpu, store, lens, 2, 64, page, seed=page + width, width=width)
+    decode_and_check(pool, gpu, 6)
+
+
+@pytest.mark.parametrize("store,D,page", [("bf16", 64, 16), ("u8_fp16", 128, 64), ("u4", 64, 32), ("fp16", 128, 1024), ("u4_fp16", 256, 16)])
+def test_decode_of_shares_of_many_pages(gpu, store, D, page):
+    """Sequences of the same pages in orders of their own: more than 4096 keys a workgroup, over the ends of pairs."""
+    B, Hkv, n = 48, 2, 24576
+    dtype, bits = STORES[store]
+    gen = torch.Generator().manual_seed(D + page)
+    one = Pool(gpu, store, [n], Hkv, D, page, seed=D)
+    pages = n // page
+    assert n % page == 0
+    order = torch.stack([torch.randperm(pages, generator=gen) for _ in range(B)])
+    lens = torch.randint(n - 4000, n + 1, (B,), generator=gen).tolist()
+    lens[3], lens[40] = 0, 5
+    table = one.table[0, :pages][order].to(torch.int32).to(gpu)
+    q = torch.randn(B, 2 * Hkv, D, generator=gen).to(dtype)
+    out, lse = one.buffers.decode(q.to(gpu), table, torch.tensor(lens, dtype=torch.int32, device=gpu), return_lse=True)
+    for b in (0, 3, 17, 40, 41, 47):
+        at = (order[b][:, None] * page + torch.arange(page)).flatten()[: lens[b]]
+        check_decode(out[b].cpu(), lse[b].cpu(), q[b], one.rows[0][0][:, at], one.rows[1][0][:, at], D**-0.5, dtype, one.spans[0][:, at] if bits else None)
+
+
+@pytest.mark.parametrize("store", ["u8", "u8_fp16", "u4", "u4_fp16"])
+def test_decode_of_scales_of_either_sign(gpu, store):
+    """(code - zero point) * scale holds for negative scales too."""
+    pool = Pool(gpu, store, [300, 70, 1], 2, 128, 16, seed=51)
+    for i in (0, 2):
+        sign = torch.randint(0, 2, pool.buffers.quant[i].shape, generator=pool.gen) * 2.0 - 1.0
+        if i == 2:
+            sign[int(pool.table[1, 0])] = -1.0  # a sequence begins with them
+            sign[int(pool.table[2, 0])] = -1.0
+        pool.buffers.quant[i].mul_(sign.to(gpu))
+        for b, n in enumerate(pool.lens):
+            for t in range(0, n, 16):
+                pool.rows[i // 2][b][:, t : t + 16] *= sign[int(pool.table[b, t // 16])][:, : min(16, n - t), None].double()
+    decode_and_check(pool, gpu, 8)
+
+
 def test_decode_without_tokens(gpu):
     pool = Pool(gpu, "bf16", [0, 0, 0], 2, 64, 16)
     pool.lens_gpu[1] = -7  # no length
@@ -529,6 +588,13 @@ def test_rotary_of_batches_and_views(gpu):
     check_rotary(first[::2, 0], one[::2, 0], 4, 2, 128, None, None, 0.0, cos, sin, positions[:2, :1], False)
     none = torch.empty(0, 1024, dtype=torch.bfloat16, device=gpu)
     rows.rotary_(none, 4, 2, 128, None, None, 0.0, cos, sin, torch.empty(0, dtype=torch.int32, device=gpu))
+
+
+def test_rotary_of_empty_batches(gpu):
+    cos, sin = rows.rope_tables(10, 64, 1e4, gpu)
+    for shape in ((0,), (2, 0), (0, 3), (3, 1, 0)):
+        x = torch.empty(*shape, 4 * 64, dtype=torch.bfloat16, device=gpu)
+        assert rows.rotary_(x, 2, 1, 64, None, None, 0.0, cos, sin, torch.empty(shape, dtype=torch.int32, device=gpu)) is x
 
 
 def test_rotary_agrees_with_the_batch_form(gpu):
