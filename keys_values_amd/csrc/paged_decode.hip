@@ -118,7 +118,8 @@ struct Rows {
       return u32x4_t{a & mask, (a >> 8) & mask, b & mask, (b >> 8) & mask};  // values 0, 2 | 1, 3 | 4, 6 | 5, 7
     }
   }
-  // A operand t of the second product: value t of each of this lane's 8 keys, in key order
+  // A operand t of the second product: value t of each of this lane's 8 keys, in key order. Of 4-bit codes the first half's are whole bytes, 16 high + low: the lower
+  // halves' sums are taken off at the end, instead of the lower halves here.
   __device__ __forceinline__ static u32x4_t v_operand(const V& r, int t) {
     u32x4_t a;
 #pragma unroll
@@ -129,7 +130,8 @@ struct Rows {
       } else {
         const int byte = U4 && t >= DPL / 2 ? t - DPL / 2 : t;
         a[jj] = __builtin_amdgcn_perm(r.w[j1][byte >> 2], r.w[j0][byte >> 2], 0x0c040c00u + 0x00010001u * (byte & 3));
-        if constexpr (U4) a[jj] &= t < DPL / 2 ? 0x00f000f0u : 0x000f000fu;
+        if constexpr (U4)
+          if (t >= DPL / 2) a[jj] &= 0x000f000fu;
       }
     }
     return a;
@@ -173,6 +175,18 @@ __device__ __forceinline__ float max_lanes(float x) {
 __device__ __forceinline__ float sum_groups(float x) {
   const u32pair_t r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// What `pair`, packed from a and b, drops of them. In fp16: a multiply-add that reads the halves where they are, exact, as the difference is.
+template <bool P16>
+__device__ __forceinline__ uint32_t dropped(uint32_t pair, float a, float b) {
+  if constexpr (P16) {
+    asm("v_fma_mix_f32 %0, %1, -1.0, %0 op_sel_hi:[1,0,0]" : "+v"(a) : "v"(pair));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(b) : "v"(pair));
+    return pack_pair<true>(a, b);
+  } else {
+    return pack_pair<false>(a - elem_lo<false>(pair), b - elem_hi<false>(pair));
+  }
 }
 
 template <typename T>
@@ -528,7 +542,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
       if constexpr (FINE) {
         u32x4_t pl;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pl[i] = pack_pair<P16>(s[2 * i] - elem_lo<P16>(pb[i]), s[2 * i + 1] - elem_hi<P16>(pb[i]));
+        for (int i = 0; i < 4; ++i) pl[i] = dropped<P16>(pb[i], s[2 * i], s[2 * i + 1]);
         if constexpr (CODES) wsum = mfma_16x16x32<true>(ones, pl, wsum);
 #pragma unroll
         for (int t = 0; t < DPL; ++t) {
@@ -573,7 +587,10 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
 #pragma unroll
       for (int t = 0; t < DPL; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] = (acc[t][i] * (U4 && t < DPL / 2 ? 0x1p20f : 0x1p24f) - corr) * unit_v;
+        for (int i = 0; i < 4; ++i) {
+          if (U4 && t < DPL / 2) acc[t][i] = ((acc[t][i] - acc[t + DPL / 2][i]) * 0x1p20f - corr) * unit_v;
+          else acc[t][i] = (acc[t][i] * 0x1p24f - corr) * unit_v;
+        }
     }
     if (again) __syncthreads();  // the results before are read
     if (m < p.Gr) {
