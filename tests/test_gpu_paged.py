@@ -597,6 +597,23 @@ def test_rotary_of_empty_batches(gpu):
         assert rows.rotary_(x, 2, 1, 64, None, None, 0.0, cos, sin, torch.empty(shape, dtype=torch.int32, device=gpu)) is x
 
 
+@pytest.mark.parametrize("interleaved,dtype", [(False, torch.bfloat16), (True, torch.float16)])
+@pytest.mark.parametrize("tokens,Hq,Hkv,D", [(7000, 32, 8, 128), (18000, 14, 2, 128), (4300, 56, 8, 128), (4400, 28, 4, 256), (16600, 28, 4, 64)])
+def test_rotary_of_many_tokens(gpu, tokens, Hq, Hkv, D, interleaved, dtype):
+    """Batches beyond the caches, bit for bit as in parts."""
+    print("rotary", tokens, Hq, Hkv, D, interleaved, flush=True)
+    gen = torch.Generator().manual_seed(tokens)
+    cos, sin = rows.rope_tables(3000, D, 1e6, gpu)
+    qw, kw = ((1 + 0.1 * torch.randn(D, generator=gen)).to(gpu) for _ in range(2))
+    whole = torch.randn(tokens, (Hq + 2 * Hkv) * D, generator=gen).to(dtype).to(gpu)
+    positions = torch.randint(-1, 3001, (tokens,), generator=gen, dtype=torch.int32).to(gpu)
+    parts = whole.clone()
+    rows.rotary_(whole, Hq, Hkv, D, qw, kw, 1e-6, cos, sin, positions, interleaved)
+    for at in range(0, tokens, 2500):
+        rows.rotary_(parts[at : at + 2500], Hq, Hkv, D, qw, kw, 1e-6, cos, sin, positions[at : at + 2500], interleaved)
+    assert torch.equal(whole.view(torch.int16), parts.view(torch.int16))
+
+
 def test_rotary_agrees_with_the_batch_form(gpu):
     """One position a batch: what qk_norm_rope_ does, but for its rounding between the steps."""
     gen = torch.Generator().manual_seed(3)
