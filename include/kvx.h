@@ -501,7 +501,8 @@ int kvx_rotary(const kvx_rotary_args* args, void* stream);
  * row layouts of enum kvx_kv_dtype (strides in elements, of codes in bytes), and for codes their scale and zero point at [p * qs_stride_page +
  * h * qs_stride_h + i] (the arrays share strides, places contiguous). A slot is p * page_size + i. The pages of a sequence, in order, are a row of a block
  * table: token t of sequence b lies in page block_table[b * bt_stride_b + t / page_size] at place t % page_size. page_size: a power of two from 16
- * to 1024. Pointers 16-byte aligned; strides of whole 16 bytes. Offsets of pages may pass 32 bits. The reference has contiguous caches only. */
+ * to 1024. Pointers 16-byte aligned; strides of whole 16 bytes, from place to place at most 2^19 elements, from page to page and from head to head below 2^31
+ * (scales: 2^30). Offsets of pages may pass 32 bits. The reference has contiguous caches only. */
 typedef struct kvx_pages {
   int32_t num_pages, page_size, Hkv, D, kv_dtype;
   void* k;
