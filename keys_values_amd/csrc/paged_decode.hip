@@ -20,10 +20,10 @@
 // w is rounded to fp16 for the product: w'. What that costs is bounded by a row's span, if the middle code c is taken out of the zero point:
 //   sum w code - sum w zp = sum w' code - c sum w' - sum w (zp - c) + sum (w - w') (code - c).
 //
-// Bounds, 16 sequences of 16384 tokens, 32 / 8 heads: plain rows are at HBM (64 values 85 us, 128 160, 256 352: 6.3, 6.7, 6.1 TB/s), 8-bit rows of 128 too (90: 6.4). 8-bit
-// rows of 64 (54: 5.6) and 4-bit ones (64 values 41, 128 54, 256 93: 4.1, 5.6, 6.2) have as much to do in the vector ALU and the address units as in memory: per
-// 32 keys of 64 values some 210 vector instructions and 12 loads. Neither fewer instructions, nor a third wavefront a SIMD, nor a second block of keys in flight
-// shortens them by more than 3 %. A call's fixed part is 5 us of serial loads (lengths, table, rows) and a join of 3 to 5, most of it the launch.
+// Bounds, 16 sequences of 16384 tokens, 32 / 8 heads: plain rows are at HBM (64 values 85 us, 128 158, 256 352: 6.3, 6.8, 6.1 TB/s), 8-bit rows of 128 too (90: 6.4). 8-bit
+// rows of 64 (52.5: 5.8) and 4-bit ones (64 values 39, 128 53, 256 92: 4.3, 5.7, 6.2) have as much to do in the vector ALU as in memory: per 32 keys of 64 4-bit
+// values some 210 vector instructions and 8 loads. Neither fewer instructions, nor a third wavefront a SIMD, nor a second block of keys in flight shortens them
+// by more than 3 %. A call's fixed part is 5 us of serial loads (lengths, table, rows) and a join of 3 to 5, most of it the launch.
 #include <type_traits>
 
 #include "key_blocks.h"
@@ -89,15 +89,35 @@ struct Rows {
   static constexpr int NL4 = D >= 128 ? D / 128 : 1;
   static constexpr int KR = U4 ? NL4 : (CODES ? D / 64 : KJ);                         // 16-byte loads per key of K
   static constexpr int VB = U4 ? DPL / 2 : DPL * ES;                                  // bytes per key of V
-  static constexpr int VW = (VB + 3) / 4;
+  // Short pieces of V rows are loaded twice as wide, by the lower eight lanes of a column group from a key and by the upper eight from the next one; then lanes
+  // exchange. 4-bit rows of 64: 41.3 -> 39.2 us, of 128 53.5 -> 53.2, 8-bit rows of 64 53.5 -> 52.5 (as below); pieces of 8 bytes gain nothing (8-bit, 128: 89.6, 89.8).
+  static constexpr bool PAIRED = CODES && VB <= 4;
+  static constexpr int VN = PAIRED ? 4 : 8, VW = PAIRED ? VB / 2 : VB / 4;  // loads, and 32-bit words of one
   // state: lane l has the scale of key l (l < 32) or the zero point of key l - 32
   struct K {
     u32x4_t w[2][KR];
     uint32_t state;
   };
   struct V {
-    uint32_t w[8][VW];
+    uint32_t w[VN][VW];
     uint32_t state;
+  };
+  // What the matrix cores take from V: the words of both keys of a pair, and the bytes of them that a lane takes
+  struct Pairs {
+    uint32_t own[VN][VW], other[PAIRED ? VN : 1][VW], pick[2];
+    __device__ __forceinline__ Pairs(const V& r, int m) {
+#pragma unroll
+      for (int j = 0; j < VN; ++j)
+#pragma unroll
+        for (int y = 0; y < VW; ++y) {
+          own[j][y] = r.w[j][y];
+          if constexpr (PAIRED) other[j][y] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)r.w[j][y], 0x128, 0xf, 0xf, true);  // row_ror:8
+        }
+      if constexpr (PAIRED) {
+        pick[0] = m < 8 ? 0x0c040c00u : 0x0c020c06u;
+        pick[1] = pick[0] + 0x00010001u;
+      }
+    }
   };
   // first d of the 8 that lane group kg supplies to matrix instruction e of the first product
   __device__ __forceinline__ static int kslice(int e, int kg) {
@@ -125,26 +145,25 @@ struct Rows {
   }
   // A operand t of the second product: value t of each of this lane's 8 keys, in key order. Of 4-bit codes the first half's are whole bytes, 16 high + low: the lower
   // halves' sums are taken off at the end, instead of the lower halves here.
-  __device__ __forceinline__ static u32x4_t v_operand(const V& r, int t) {
+  __device__ __forceinline__ static u32x4_t v_operand(const Pairs& r, int t) {
     u32x4_t a;
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) {
-      const int j0 = 2 * jj, j1 = 2 * jj + 1;
-      if constexpr (!CODES) {
-        a[jj] = __builtin_amdgcn_perm(r.w[j1][t >> 1], r.w[j0][t >> 1], (t & 1) ? 0x07060302u : 0x05040100u);
-      } else {
-        const int byte = U4 && t >= DPL / 2 ? t - DPL / 2 : t;
-        a[jj] = __builtin_amdgcn_perm(r.w[j1][byte >> 2], r.w[j0][byte >> 2], 0x0c040c00u + 0x00010001u * (byte & 3));
-        if constexpr (U4)
-          if (t >= DPL / 2) a[jj] &= 0x000f000fu;
-      }
+      const int j0 = 2 * jj, j1 = 2 * jj + 1, byte = U4 && t >= DPL / 2 ? t - DPL / 2 : t;
+      if constexpr (!CODES) a[jj] = __builtin_amdgcn_perm(r.own[j1][t >> 1], r.own[j0][t >> 1], (t & 1) ? 0x07060302u : 0x05040100u);
+      else if constexpr (PAIRED) a[jj] = __builtin_amdgcn_perm(r.other[jj][byte >> 1], r.own[jj][byte >> 1], r.pick[byte & 1]);
+      else a[jj] = __builtin_amdgcn_perm(r.own[j1][byte >> 2], r.own[j0][byte >> 2], 0x0c040c00u + 0x00010001u * (byte & 3));
+      if constexpr (U4)
+        if (t >= DPL / 2) a[jj] &= 0x000f000fu;
     }
     return a;
   }
   // d of row `mrow` of matrix instruction t of the second product
   __device__ __forceinline__ static int dmap(int t, int mrow) {
-    if constexpr (U4) return t < DPL / 2 ? (DPL / 2) * mrow + t : D / 2 + (DPL / 2) * mrow + (t - DPL / 2);
-    else return DPL * mrow + t;
+    const int u = U4 && t >= DPL / 2 ? t - DPL / 2 : t, first = U4 && t >= DPL / 2 ? D / 2 : 0;
+    constexpr int EACH = U4 ? DPL / 2 : DPL;  // values of a row's piece, or bytes
+    if constexpr (PAIRED) return first + 2 * EACH * (mrow & 7) + 4 * (u >> 1) + 2 * (mrow >> 3) + (u & 1);
+    else return first + EACH * mrow + u;
   }
 };
 
@@ -280,7 +299,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
     return s;
   };
 
-  const uint32_t k_lane = (uint32_t)m * p.k_row + (U4 && D == 64 ? 8 : 16) * kg, v_lane = 4 * kg * p.v_row + (uint32_t)m * R::VB;
+  const uint32_t k_lane = (uint32_t)m * p.k_row + (U4 && D == 64 ? 8 : 16) * kg, v_lane = R::PAIRED ? (4 * kg + (m >> 3)) * p.v_row + (m & 7) * 2 * R::VB : 4 * kg * p.v_row + m * R::VB;
 
   // ---- rows of a block of 32 keys. Lane 2 j + gi holds the page of half gi of the wavefront's block j (of 32 at a time). A page that the pool does not have is
   // read as page 0, and its keys are masked behind. Keys behind the end lie in the same pages, or masked ones.
@@ -344,22 +363,20 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
       const uint8_t* base = v_head + (uint64_t)(uint32_t)t.page(gi) * p.v_page;
       const uint32_t off = (uint32_t)((chunk + 16 * gi) & mask) * p.v_row + v_lane;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* row = base + (off + (uint32_t)i * p.v_row);
-        uint32_t(&x)[R::VW] = r.w[4 * gi + i];
-        if constexpr (R::VB >= 16) {
+      for (int i = 0; i < R::VN / 2; ++i) {
+        const uint8_t* row = base + (off + (uint32_t)(8 / R::VN * i) * p.v_row);
+        uint32_t(&x)[R::VW] = r.w[R::VN / 2 * gi + i];
+        if constexpr (R::VW >= 4) {
 #pragma unroll
-          for (int y = 0; y < R::VB / 16; ++y) {
+          for (int y = 0; y < R::VW / 4; ++y) {
             const u32x4_t z = once<u32x4_t>(row + 16 * y);
             x[4 * y] = z[0]; x[4 * y + 1] = z[1]; x[4 * y + 2] = z[2]; x[4 * y + 3] = z[3];
           }
-        } else if constexpr (R::VB == 8) {
+        } else if constexpr (R::VW == 2) {
           const u32x2_t z = once<u32x2_t>(row);
           x[0] = z[0]; x[1] = z[1];
-        } else if constexpr (R::VB == 4) {
-          x[0] = once<uint32_t>(row);
         } else {
-          x[0] = (uint32_t)once<uint16_t>(row);
+          x[0] = once<uint32_t>(row);
         }
       }
     }
@@ -544,6 +561,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
       const u32x4_t pb = {pack_pair<P16>(s[0], s[1]), pack_pair<P16>(s[2], s[3]), pack_pair<P16>(s[4], s[5]), pack_pair<P16>(s[6], s[7])};
       const u32x4_t ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
       if constexpr (CODES) wsum = mfma_16x16x32<true>(ones, pb, wsum);
+      const typename R::Pairs rows(v, m);
       if constexpr (FINE) {
         u32x4_t pl;
 #pragma unroll
@@ -551,12 +569,12 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
         if constexpr (CODES) wsum = mfma_16x16x32<true>(ones, pl, wsum);
 #pragma unroll
         for (int t = 0; t < DPL; ++t) {
-          const u32x4_t x = R::v_operand(v, t);
+          const u32x4_t x = R::v_operand(rows, t);
           acc[t] = mfma_16x16x32<P16>(x, pl, mfma_16x16x32<P16>(x, pb, acc[t]));
         }
       } else {
 #pragma unroll
-        for (int t = 0; t < DPL; ++t) acc[t] = mfma_16x16x32<P16>(R::v_operand(v, t), pb, acc[t]);
+        for (int t = 0; t < DPL; ++t) acc[t] = mfma_16x16x32<P16>(R::v_operand(rows, t), pb, acc[t]);
       }
     };
 
@@ -599,7 +617,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
     }
     if (again) __syncthreads();  // the results before are read
     if (m < p.Gr) {
-      constexpr int RUN = U4 && D == 64 ? 2 : 4;  // values side by side
+      constexpr int RUN = R::PAIRED ? 2 : 4;  // values side by side
       typedef float run_t __attribute__((ext_vector_type(RUN)));
 #pragma unroll
       for (int i = 0; i < 4; ++i)
