@@ -583,7 +583,9 @@ static int check_paged_decode(const kvx_paged_decode_args* a) {
   KVX_REQUIRE(a->Hq > 0 && a->Hq % a->pages.Hkv == 0, KVX_ERR_INVALID, "%s: Hq=%d must be a positive multiple of Hkv=%d", who, a->Hq, a->pages.Hkv);
   KVX_REQUIRE(a->Hq / a->pages.Hkv <= 16, KVX_ERR_UNSUPPORTED, "%s: %d query heads per KV head (at most 16)", who, a->Hq / a->pages.Hkv);
   const int64_t units = (int64_t)a->B * a->pages.Hkv * (((int64_t)a->max_pages * a->pages.page_size + 127) / 128);
-  KVX_REQUIRE(units < ((int64_t)1 << 30), KVX_ERR_UNSUPPORTED, "%s: %d sequences of %d pages, %d KV heads: beyond 2^30 shares of 128 tokens", who, a->B, a->max_pages,
+  // pairs of codes count for up to two shares more, in 32 bits
+  KVX_REQUIRE(units < ((int64_t)1 << 30) && units + 2 * (int64_t)a->B * a->pages.Hkv <= INT32_MAX, KVX_ERR_UNSUPPORTED,
+              "%s: %d sequences of %d pages, %d KV heads: beyond 2^30 shares of 128 tokens", who, a->B, a->max_pages,
               a->pages.Hkv);
   KVX_REQUIRE(a->sm_scale > 0.0f, KVX_ERR_INVALID, "%s: sm_scale must be positive", who);
   return KVX_OK;

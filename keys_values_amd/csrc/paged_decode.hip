@@ -40,7 +40,7 @@ struct PagedParams {
   const int* lens;
   const int* table;
   int64_t table_sb;
-  int B, Hkv, cap /* tokens of a table's pages */, unit /* log2 of the keys of a unit */, cus /* compute units */, workgroups, shift /* log2 of the page size */, max_pages;
+  int B, Hkv, cap /* tokens of a table's pages */, unit /* log2 of the keys of a unit */, cus /* compute units */, workgroups, extra /* units added to a pair */, shift /* log2 of the page size */, max_pages;
   int num_pages, Gr /* query heads per KV head */;
 
   const uint16_t* q;
@@ -59,7 +59,8 @@ struct PagedParams {
   int* part_of;    // by pairs: the workgroup that left a pair's first partial; by workgroups: the pair; and how many partials the pair has, 0: none. NULL: no partials
 };
 
-__device__ __forceinline__ int units_of(int len, int cap, int unit) { return max(1, (min(max(len, 0), cap) + (1 << unit) - 1) >> unit); }
+// Units of a pair of `len` tokens: those with keys, and, behind them, as many without as the change to the pair takes the time of.
+__device__ __forceinline__ int units_of(int len, const PagedParams& p, int extra) { return max(1, (min(max(len, 0), p.cap) + (1 << p.unit) - 1) >> p.unit) + extra; }
 
 // Inclusive sum over the lanes of a wavefront, on the vector ALU.
 __device__ __forceinline__ int scan(int x) {
@@ -237,24 +238,24 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
   __shared__ float red_m[WAVES][16], red_l[WAVES][16];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, kg = lane >> 4;
-  const int B = p.B, Hkv = p.Hkv, w = blockIdx.x, mask = (1 << p.shift) - 1;
+  const int B = p.B, Hkv = p.Hkv, w = blockIdx.x, mask = (1 << p.shift) - 1, extra = CODES ? p.extra : 0;
 
   // ---- this workgroup's units: every wavefront finds them for itself, 64 sequences at a time
   const int windows = (B + 63) / 64;
   auto window = [&](int i) { return 64 * i + lane < B ? p.lens[64 * i + lane] : -1; };
-  auto units_in = [&](int len, int i) { return 64 * i + lane < B ? units_of(len, p.cap, p.unit) : 0; };
+  auto units_in = [&](int len, int i) { return 64 * i + lane < B ? units_of(len, p, extra) : 0; };
   int lane_len = 0, mine = 0;  // lane_len: of sequence (b & ~63) + lane
   for (int i = 0; i < windows; ++i) {
     lane_len = window(i);
     mine += units_in(lane_len, i);
   }
   const int total = __builtin_amdgcn_readlane(scan(mine), 63) * Hkv;
-  // Workgroups that share the units, of the grid's three a compute unit: all where pairs are short (of up to four units on average; B256, 32 / 8 heads of 128, 50 to 400
+  // Workgroups that share the units, of the grid's two or three a compute unit: all where pairs are short (of up to four units on average; B256, 32 / 8 heads of 128, 50 to 400
   // tokens: 42.7 us, 44.4 with two a compute unit, 54.2 with one), two elsewhere (64 sequences of 1 to 8192, 28 / 4 heads: 30.9, 33.3 with one, 32.1 with three), and
   // one, whose partials are the fewest, where pairs are long and rows of 128 bytes and more keep enough of them on their way (16 x 16384, plain rows of 128: 158.3, 162.0
   // with two, 165.6 with three; but 4-bit rows of 128: 65.7, 53.7 with two).
   constexpr bool WIDE = D * ES >= (U4 ? 256 : 128);
-  const int pairs = B * Hkv, sharing = (total + 3) / 4 <= pairs ? p.workgroups : WIDE && total / 64 >= pairs ? p.cus : 2 * p.cus;
+  const int pairs = B * Hkv, full = total - pairs * extra, sharing = (full + 3) / 4 <= pairs ? p.workgroups : WIDE && full / 64 >= pairs ? p.cus : 2 * p.cus;
   const Shares shares(total, min(sharing, p.workgroups));
   int unit = shares.first(w);  // the next unit
   const int end = shares.first(w + 1);
@@ -279,23 +280,31 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
   struct Stretch {
     int b, h, begin, units, first, n, k_begin, k_end;
   };
+  auto go_to = [&](int to, int units) {  // to a unit of the same pair, or the next one's first
+    unit = to;
+    if (unit == begin_b + units * Hkv) {
+      begin_b = unit;
+      ++b;
+      if ((b & 63) == 0 && b < B) lane_len = window(b >> 6);
+    }
+  };
+  if constexpr (CODES) {  // a share does not begin with units without keys
+    const int units = units_of(__builtin_amdgcn_readlane(lane_len, b & 63), p, extra), left = units - (unit - begin_b) % units;
+    if (left <= extra) go_to(unit + left, units);
+    if (unit >= end) return;
+  }
   auto take = [&] {
     Stretch s;
     const int len = min(max(__builtin_amdgcn_readlane(lane_len, b & 63), 0), p.cap);
     s.b = b;
-    s.units = units_of(len, p.cap, p.unit);
+    s.units = units_of(len, p, extra);
     s.h = (unit - begin_b) / s.units;
     s.begin = begin_b + s.h * s.units;
     s.first = unit - s.begin;
     s.n = min(s.units - s.first, end - unit);
     s.k_begin = s.first << p.unit;
     s.k_end = min(len, (s.first + s.n) << p.unit);
-    unit += s.n;
-    if (unit == begin_b + s.units * Hkv) {
-      begin_b = unit;
-      ++b;
-      if ((b & 63) == 0 && b < B) lane_len = window(b >> 6);
-    }
+    go_to(unit + s.n, s.units);
     return s;
   };
 
@@ -634,7 +643,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
       }
     }
     __syncthreads();
-    const bool alone = now.first == 0 && now.n == now.units;  // the pair is this workgroup's alone
+    const bool alone = now.first == 0 && now.n >= now.units - extra;  // the pair is this workgroup's alone
     const int slot = 2 * w + (now.first == 0 ? 1 : 0);
     auto sums = [&](int g, float (&f)[WAVES], float& top) {
       top = red_m[0][g];
@@ -667,7 +676,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
     if (tid == 0 && p.part_of && now.first == 0 && (p.by_pair || !alone)) {
       const int pair = now.b * Hkv + now.h, i = 2 * (p.by_pair ? pair : w);
       p.part_of[i] = p.by_pair ? w : pair;
-      p.part_of[i + 1] = alone ? 0 : shares.owner(now.begin + now.units - 1) - w + 1;
+      p.part_of[i + 1] = alone ? 0 : shares.owner(now.begin + now.units - extra - 1) - w + 1;
     }
     if (!more) break;
   }
@@ -772,10 +781,15 @@ PagedParams params_of(const kvx_paged_decode_args& a) {
   p.lse = a.lse;
   // Tables of up to 512 tokens: a pair is a workgroup's, and there is no second launch.
   p.unit = p.cap <= 4 * UNIT ? 9 : 7;
+  // Beginning a pair of codes takes the time of one unit of 8-bit rows, or two of 4-bit ones: it counts as such, or the workgroups that get the short pairs come last. 92
+  // sequences of lengths even in the logarithm from 15 to 9560, 4-bit rows of 128, 32 / 4 heads: 40.8 us without, 29.6 with one unit, 26.2 with two; 14 from 25 to 35609, 8-bit
+  // rows of 256: 76.8 without, 63.1 with one or two. Plain rows, whose units take longer, only lose: 200 of 1 to 3000, 65.8 without, 68.5 with one.
+  p.extra = plain || p.unit == 9 ? 0 : kv_is_u4(g.kv_dtype) ? 2 : 1;
   p.cus = num_cus();
   // One workgroup a compute unit for the only pair: the partials of more take longer to join than they save (one of 100000 tokens, 16 heads of 128: 21.7 us, 33.8
   // with three).
-  const int64_t per_cu = g.D == 256 ? waves_per_simd(256, !plain) : 3;
+  // More of them than registers leave room for would come in a second round: 239 sequences of 1 to 641, 24 / 8 heads of 128, 8-bit: 28.7, 35.7 with three.
+  const int64_t per_cu = g.D == 256 ? waves_per_simd(256, !plain) : g.D == 128 && !plain && !kv_is_u4(g.kv_dtype) ? 2 : 3;
   const int64_t pairs = (int64_t)a.B * a.pages.Hkv, units = pairs * ((p.cap + (1 << p.unit) - 1) >> p.unit), most = p.cus * (pairs < per_cu ? pairs : per_cu);
   p.workgroups = (int)(units < most ? units : most);
   p.by_pair = pairs <= p.workgroups;
