@@ -13,7 +13,8 @@ written twice in one call.
 A layer's step for one new token a sequence is ``longctx.ops.rotary_``, ``paged_write``, ``attention.ops.paged_decode``; a later
 chunk of a prompt attends over ``paged_read`` rows with ``attention.ops.prefill_core``. Tables, lengths, slots and positions
 stay on the device and are read by the kernels alone, so the calls can be captured into a graph and replayed with others in
-their place. There is no CPU path.
+their place (graphs that share a memory pool in the order of their capture, as torch asks for: a later one's tensors may lie where
+an earlier one had its workspace). There is no CPU path.
 """
 from typing import Optional, Tuple
 

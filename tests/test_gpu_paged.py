@@ -708,6 +708,35 @@ def test_captured_steps(gpu, store):
         assert torch.equal(again[0], out) and torch.equal(again[1], lse)  # the eager result
 
 
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("store", ["fp16", "u8_fp16", "u4"])
+def test_two_captured_steps_in_turn(gpu, store, shared):
+    """Two graphs, replayed in either order on a stream of their own, each before the other's results are looked at. Of one memory pool in the order of their
+    capture only, as torch asks for: the second graph's results may lie where the first one's workspace was."""
+    layers = [Layer(gpu, store, lens, 6, 2, 64, 32, 24 + i) for i, lens in enumerate(([900, 33, 0], [5, 1500]))]
+    graphs, results, pool = [], [], None
+    for layer in layers:
+        layer.next()
+        layer.step()
+        torch.cuda.synchronize()
+        layer.next()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=pool):
+            results.append(layer.step())
+        pool = graphs[0].pool() if shared else None
+    stream = torch.cuda.Stream()
+    for order in ((0, 1),) * 4 if shared else ((0, 1), (1, 0), (0, 1), (1, 0)):
+        for i in order:
+            layers[i].next()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for i in order:
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for layer, (out, lse) in zip(layers, results):
+            layer.check(out, lse)
+
+
 def test_a_later_chunk_of_a_prompt(gpu):
     """A chunk attends over the rows read back, as over a contiguous cache."""
     gen = torch.Generator().manual_seed(31)
