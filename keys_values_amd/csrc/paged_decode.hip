@@ -15,7 +15,8 @@
 // Codes. (code - zp) * scale is linear in the code, so the codes themselves are the operands, and scale and zero point are applied to a key's 16 logits and weights
 // instead of its 2 D values: 16-bit integers below 1024 are what fp16 calls subnormal numbers, code * 2^-24, which the matrix cores multiply exactly,
 // so one byte permute makes two operand values of 8-bit codes, and one mask, for 4-bit ones, the codes of the high halves as 16 times theirs.
-//   logit = scale_k (S - zp_k sum q),        S = sum code q,      q in fp16 times a power of two that brings the head's largest below 2^15 (exact)
+//   logit = scale_k (S - zp_k sum q),        S = sum code q,      q in fp16 times a power of two that brings the head's largest below 2^15 (exact, but for what
+//                                                                 is 2^24 times smaller than it: that is off by 2^-35 of it at most)
 //   o     = (sum w code - sum w zp_v) / l,   w = p scale_v,       in units of a power of two above the largest scale_v so far
 // w is rounded to fp16 for the product: w'. What that costs is bounded by a row's span, if the middle code c is taken out of the zero point:
 //   sum w code - sum w zp = sum w' code - c sum w' - sum w (zp - c) + sum (w - w') (code - c).
@@ -433,13 +434,13 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
       next_page = pages_of(next, 0);
     }
 
-    float qsum = 0.0f, to_logit = p.c;
+    float qsum = 0.0f, to_logit = 1.0f;  // to_logit: a power of two, of the head's, so that products with it are exact
     // Columns beyond the group are zeros: with copies of the last head there the matrix cores are slower (16 x 16384, 32 / 8 heads of 64, plain: 84.5 us, 90.5)
 #pragma unroll
     for (int e = 0; e < KJ; ++e)
       if (m >= p.Gr) qb[e] = u32x4_t{0u, 0u, 0u, 0u};
     if constexpr (CODES) {
-      auto largest = [&](bool finite) {  // of the group's queries
+      auto largest = [&](bool finite) {  // of the head's values: heads of a group may differ by more than fp16 spans
         float top = 0.0f;
 #pragma unroll
         for (int e = 0; e < KJ; ++e)
@@ -449,14 +450,14 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
             top = fmaxf(top, finite && !(x0 < INFINITY) ? 0.0f : x0);
             top = fmaxf(top, finite && !(x1 < INFINITY) ? 0.0f : x1);
           }
-        return max_lanes(top);
+        return max_halves(max_row_pairs(top));
       };
       float top = largest(false);
-      if (!(top < INFINITY)) top = largest(true);
+      if (__any(!(top < INFINITY))) top = largest(true);
       // 2^x that brings it to [2^14, 2^15)
       const int ex = (int)(__float_as_uint(top) >> 23), up = ex == 0 ? 127 : min(268 - ex, 253);
       const float by = __uint_as_float((uint32_t)up << 23);
-      to_logit = __uint_as_float((uint32_t)(254 - up) << 23) * p.c * 0x1p24f;
+      to_logit = __uint_as_float((uint32_t)(254 - up) << 23);
 #pragma unroll
       for (int e = 0; e < KJ; ++e) {
         float x[8];
@@ -488,7 +489,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
     auto whole = [&](int chunk) { return chunk + 32 <= now.k_end && t.ok0 && t.ok1; };
     // key `i` of half gi is one of the sequence's
     auto live = [&](int chunk, int gi, int i) { return t.ok(gi) && chunk + 16 * gi + i < now.k_end; };
-    // logits in log2 units: head m, keys 4 kg + i of the two halves
+    // logits: head m, keys 4 kg + i of the two halves; in log2 units, of codes by to_logit, which is the head's
     auto logits = [&](int chunk, float (&s)[8]) {
       f32x4_t x[2];
 #pragma unroll
@@ -498,12 +499,12 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
         for (int e = 0; e < KJ; ++e) x[gi] = mfma_16x16x32<P16>(R::k_operand(k, gi, e), qb[e], x[gi]);
       }
       if constexpr (CODES) {
-        const State st(state[wave][0], lane < 32 ? __uint_as_float(k.state) * to_logit : (float)(int32_t)k.state, lane, kg);
+        const State st(state[wave][0], lane < 32 ? __uint_as_float(k.state) * (p.c * 0x1p24f) : (float)(int32_t)k.state, lane, kg);
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[i] = fmaf(st.zp[i >> 2][i & 3], qsum, x[i >> 2][i & 3]) * st.scale[i >> 2][i & 3];
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = x[i >> 2][i & 3] * to_logit;
+        for (int i = 0; i < 8; ++i) s[i] = x[i >> 2][i & 3] * p.c;
       }
       if (!whole(chunk)) {
 #pragma unroll
@@ -515,6 +516,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
       float top = s[0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
+      if constexpr (CODES) top *= to_logit;
       if (__any(top > m_run + kTop)) {
         top = max_halves(max_row_pairs(top));  // of the head, over the four lane groups
         const bool moves = top > m_run + kTop;
@@ -530,7 +532,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        s[i] = fast_exp2(s[i] - m_run);
+        s[i] = fast_exp2(CODES ? fmaf(s[i], to_logit, -m_run) : s[i] - m_run);
         l_run += s[i];
       }
     };
