@@ -24,3 +24,49 @@ def test_heads_of_a_group_of_very_different_queries(gpu, store, D):
     got, got_lse = pool.buffers.decode(alone.to(gpu), pool.table_gpu, pool.lens_gpu, return_lse=True)
     keep = [0, 2, 3, 5, 6, 7, 8, 10, 11, 13, 14, 15]
     assert torch.equal(got[:, keep], out[:, keep]) and torch.equal(got_lse[:, keep], lse[:, keep])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("store", ["u8_fp16", "u4_fp16"])
+def test_codes_beside_rows_of_large_scales(gpu, store, D):
+    """V rows of zeros with a scale 2^10 times that of the others, every fourth: code and zero point in the middle. They have no part in the outputs, and what is multiplied
+    with them must not cut the others' products short: a product of 2^10 w with a bare code, a subnormal number of exponent -14, would cut those with w at 2^-24 2^-14
+    2^10, a sixteenth of a code.
+
+    Weights are all equal (q = 0). In units of a small row's scale times its codes: a weight in two parts of fp16 is off by 2^-20 of itself at most (its second part may
+    be subnormal, 2^-25 where the first is 2^-4 or more). Products are cut at 2^-24 of the largest of 8; one rounding of 2^-24 for each of the sums of 8 and of the joins, 72
+    with those of the zero points' part. All of them relative to sum w (half the codes), of 4-bit codes' first half, which are whole bytes over 16, 9 / 8 of it."""
+    pool = Pool(gpu, store, [96, 31], 2, D, 16, seed=D)
+    bits, buffers = pool.bits, pool.buffers
+    mid, packed = (8, 0x88) if bits == 4 else (128, 128)
+    small = buffers.quant.v_scale.clone()
+    buffers.v[:, :, ::4] = packed
+    buffers.quant.v_zp[:, :, ::4] = mid
+    buffers.quant.v_scale[:, :, ::4] *= 2.0**10
+    q = torch.zeros(2, 4, D, dtype=pool.dtype)
+    out, _ = buffers.decode(q.to(gpu), pool.table_gpu, pool.lens_gpu)
+    for b, n in enumerate(pool.lens):
+        values = pool.rows[1][b].clone()
+        values[:, ::4] = 0.0
+        ref = values.mean(1).repeat_interleave(2, 0)
+        half = small.cpu()[pool.table[b, : -(-n // 16)].long()].transpose(0, 1).flatten(1)[:, :n].clone()
+        half[:, ::4] = 0.0
+        half = (half * 2.0 ** (bits - 1) * 1.125).double().mean(1).repeat_interleave(2, 0)[:, None]
+        tol = 2.0**-11 * ref.abs() + half * (2.0**-20 + 80 * 2.0**-24) * (1 + 2.0**-11) + 2.0**-25
+        err = (out[b].double().cpu() - ref).abs()
+        assert (err <= tol).all(), f"off by {(err / tol).max().item():.2f} tolerances"
+
+
+@pytest.mark.parametrize("store,Hq,D,factor", [("u4_fp16", 16, 64, 1.0), ("u4_fp16", 8, 128, 0.01), ("u8_fp16", 8, 128, 1.0), ("u8_fp16", 4, 256, 0.3)])
+def test_long_sequences_of_codes_are_off_by_the_outputs_rounding(gpu, store, Hq, D, factor):
+    """Root mean square over the outputs: the rounding to fp16 of the 64-bit result, and at most a fifth of that beside it (in quadrature, 1.02). One sequence is shared by all
+    compute units, four wavefronts each, so 50000 keys are some 100 roundings of fp32 to a wavefront, with the joins: 100^(1/2) 2^-25 of sums that are, without the middle
+    code, about |v| n^(-1/2), as the outputs are: a thousandth of the outputs' rounding. The weights' logits are off by D^(1/2) 2^-24 |q k| in the mean, 2^-18, which moves
+    outputs by less than 2^-18, where the outputs' rounding is 2^-12."""
+    n = 50000
+    pool = Pool(gpu, store, [n], 1, D, 64, seed=D)
+    q = (factor * torch.randn(1, Hq, D, generator=pool.gen)).to(pool.dtype)
+    out, _ = pool.buffers.decode(q.to(gpu), pool.table_gpu, pool.lens_gpu)
+    ref = torch.softmax(q[0].double() @ pool.rows[0][0][0].T * D**-0.5, -1) @ pool.rows[1][0][0]
+    off, rounding = ((x.double().cpu() - ref).norm().item() for x in (out[0], ref.to(pool.dtype)))
+    assert off <= 1.02 * rounding, f"{off / rounding:.4f} times the rounding"
