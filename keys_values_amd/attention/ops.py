@@ -167,7 +167,7 @@ def paged_decode(
 
     Group sizes 1 to 16 for every store and head size. Pages of codes (``quant`` given) stand for ``(code - zero point) * scale``: what
     ``decode_core`` rounds to the query's type before it multiplies is not rounded here. Rows of the pages behind a
-    sequence's end may hold anything."""
+    sequence's end may hold anything. An infinite value in one of its plain rows makes that output infinite."""
     return _lib.host().paged_decode(query, key_pages, value_pages, block_table, lens, scale, return_lse, quant)
 
 

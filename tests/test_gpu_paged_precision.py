@@ -1,5 +1,7 @@
 """How exact attention of one token over pages is, where looser bounds would not show a part of the arithmetic that is missing or cut off, against the same
 mathematics in 64 bits."""
+import math
+
 import pytest
 import torch
 from test_gpu_paged import Pool, decode_and_check
@@ -70,3 +72,62 @@ def test_long_sequences_of_codes_are_off_by_the_outputs_rounding(gpu, store, Hq,
     ref = torch.softmax(q[0].double() @ pool.rows[0][0][0].T * D**-0.5, -1) @ pool.rows[1][0][0]
     off, rounding = ((x.double().cpu() - ref).norm().item() for x in (out[0], ref.to(pool.dtype)))
     assert off <= 1.02 * rounding, f"{off / rounding:.4f} times the rounding"
+
+
+def by_hand(pool, q, b):
+    """The outputs' terms p v in 64 bits, (Hq, n, D): of weights that are all positive, so that an infinite value is not multiplied by 0."""
+    keys, values = (pool.rows[i][b].repeat_interleave(q.shape[1] // pool.Hkv, 0) for i in (0, 1))
+    p = torch.softmax((keys @ q[b].double()[..., None])[..., 0] * pool.D**-0.5, -1)
+    assert (p > 0).all()
+    return p[..., None] * values
+
+
+@pytest.mark.parametrize("lens,page", [([1, 2, 300, 40], 16), ([20000, 1, 3], 64)])
+@pytest.mark.parametrize("store,D", [("bf16", 64), ("bf16", 128), ("bf16", 256), ("fp16", 64), ("fp16", 128), ("fp16", 256)])
+def test_infinite_values(gpu, store, D, lens, page):
+    """A live key's infinite value makes its column infinite, with any weight; two of either sign, or a NaN, make it NaN. Other columns are what they are without."""
+    print("infinite", store, D, lens, flush=True)
+    pool = Pool(gpu, store, lens, 2, D, page, seed=D)
+    q = (3.0 * torch.randn(len(lens), 8, D, generator=pool.gen)).to(pool.dtype)
+    plain, _ = pool.buffers.decode(q.to(gpu), pool.table_gpu, pool.lens_gpu)
+    for b, n in enumerate(lens):
+        for j, t in enumerate(sorted({0, n // 3, n // 2, n - 1})):  # some of them with weights that 16 bits do not hold
+            at = (int(pool.table[b, t // page]), j % 2, t % page)
+            for column, value in ((7 * j, math.inf), (7 * j + 1, -math.inf), (3, (-1.0) ** (j // 2) * math.inf), (D - 1 - j, math.nan)):
+                pool.buffers.v[(*at, column)] = value
+                pool.rows[1][b][j % 2, t, column] = value
+    out, lse = pool.buffers.decode(q.to(gpu), pool.table_gpu, pool.lens_gpu, return_lse=True)
+    assert torch.isfinite(lse).all()
+    got, plain = out.double().cpu(), plain.double().cpu()
+    for b in range(len(lens)):
+        want = by_hand(pool, q, b).sum(1)
+        infinite, finite = torch.isinf(want), torch.isfinite(want)
+        assert torch.equal(torch.isnan(got[b]), torch.isnan(want)) and infinite.any() and finite.any()
+        assert torch.equal(got[b][infinite], want[infinite]) and torch.equal(got[b][finite], plain[b][finite])
+
+
+@pytest.mark.parametrize("store", ["u8", "u4_fp16"])
+def test_infinite_scales(gpu, store):
+    """Rows of codes whose scale is not finite make their heads' outputs infinite or NaN, and no others."""
+    pool = Pool(gpu, store, [100, 31], 2, 64, 16, seed=5)
+    q = torch.randn(2, 4, 64, generator=pool.gen).to(pool.dtype).to(gpu)
+    before = pool.buffers.decode(q, pool.table_gpu, pool.lens_gpu)[0]
+    pool.buffers.quant.v_scale[int(pool.table[0, 2]), 1, 3] = math.inf
+    out = pool.buffers.decode(q, pool.table_gpu, pool.lens_gpu)[0]
+    assert not torch.isfinite(out[0, 2:]).any() and torch.equal(out[0, :2], before[0, :2]) and torch.equal(out[1], before[1])
+
+
+@pytest.mark.parametrize("store", ["bf16", "fp16", "u8", "u4_fp16"])
+def test_infinite_values_in_masked_places(gpu, store):
+    """Of tokens in pages that the pool does not have, and behind the end."""
+    pool = Pool(gpu, store, [100, 31], 1, 64, 16, seed=5)
+    q = torch.randn(2, 4, 64, generator=pool.gen).to(pool.dtype).to(gpu)
+    pool.table_gpu[0, 2] = -1
+    before = pool.buffers.decode(q, pool.table_gpu, pool.lens_gpu)[0]
+    for p, places in ((int(pool.table[0, 2]), slice(0, 16)), (int(pool.table[0, 6]), slice(4, 16)), (int(pool.table[1, 1]), slice(15, 16))):
+        if pool.bits is None:
+            pool.buffers.v[p, 0, places] = math.inf
+        else:
+            pool.buffers.quant.v_scale[p, 0, places] = math.inf
+    after = pool.buffers.decode(q, pool.table_gpu, pool.lens_gpu)[0]
+    assert torch.isfinite(before).all() and torch.equal(before, after)
