@@ -518,7 +518,8 @@ typedef struct kvx_pages {
 
 /* Write `tokens` new rows: row t of key and value, (tokens, Hkv, D) of the store's element type by strides, to slot slots[t] (int64), quantised on the way in
  * as kvx_quantize_rows does where the pages hold codes. A negative slot, or one behind the pool's last, is no slot: the row is dropped (padding). Two rows
- * of one call with the same slot: one of them is stored, or parts of each. */
+ * of one call with the same slot: one of them is stored, or parts of each. A call takes fewer than 2^23 groups of 2048 / D rows: of tokens * Hkv plain rows, of codes
+ * Hkv times the groups of tokens. */
 typedef struct kvx_paged_write_args {
   kvx_pages pages;
   int64_t tokens;
@@ -532,7 +533,8 @@ int kvx_paged_write(const kvx_paged_write_args* args, void* stream);
 
 /* Rows of sequences back, dequantised where the pages hold codes: key / value, (B, Hkv, length, D) of the store's element type by strides, get the first
  * min(lens[b], length) rows of sequence b, and zeros behind them. Rows of pages that the pool does not have, and of tokens behind
- * max_pages * page_size, are zeros too. */
+ * max_pages * page_size, are zeros too. B is at most 65535; a call takes fewer than 2^23 groups of 2048 / D rows,
+ * B * Hkv times the groups of length. */
 typedef struct kvx_paged_read_args {
   kvx_pages pages;
   int32_t B, length, max_pages;

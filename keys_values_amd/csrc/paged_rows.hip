@@ -157,12 +157,20 @@ int launch_paged_write(const kvx_paged_write_args& a, hipStream_t st) {
 
 int launch_paged_read(const kvx_paged_read_args& a, hipStream_t st) {
   const int64_t each = NTHREADS / (a.pages.D / 8), grid = (a.length + each - 1) / each, pairs = (int64_t)a.B * a.pages.Hkv;
-  KVX_REQUIRE(pairs <= 65535 && grid * pairs < (1 << 23), KVX_ERR_UNSUPPORTED, "kvx_paged_read: %lld (sequence, head) pairs of %d tokens in one call", (long long)pairs,
-              a.length);
-  by_store(a.pages, [&](auto d, auto kv) {
-    hipLaunchKernelGGL((paged_read_kernel<decltype(d)::value, decltype(kv)::value>), dim3((unsigned)grid, (unsigned)pairs), dim3(NTHREADS), 0, st, a,
-                       __builtin_ctz(a.pages.page_size));
-  });
+  KVX_REQUIRE(grid * pairs < (1 << 23), KVX_ERR_UNSUPPORTED, "kvx_paged_read: %lld (sequence, head) pairs of %d tokens in one call", (long long)pairs, a.length);
+  const int most = 65535 / a.pages.Hkv;  // sequences of a launch: a grid's y counts to 65535
+  for (int done = 0; done < a.B; done += most) {
+    kvx_paged_read_args part = a;
+    part.B = min(most, a.B - done);
+    part.block_table += done * a.bt_stride_b;
+    part.lens += done;
+    part.key = (uint16_t*)a.key + done * a.key_stride_b;
+    part.value = (uint16_t*)a.value + done * a.value_stride_b;
+    by_store(a.pages, [&](auto d, auto kv) {
+      hipLaunchKernelGGL((paged_read_kernel<decltype(d)::value, decltype(kv)::value>), dim3((unsigned)grid, (unsigned)(part.B * a.pages.Hkv)), dim3(NTHREADS), 0, st, part,
+                         __builtin_ctz(a.pages.page_size));
+    });
+  }
   KVX_HIP(hipGetLastError());
   return KVX_OK;
 }
