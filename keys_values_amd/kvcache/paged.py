@@ -10,8 +10,9 @@ sequence ``b`` lies in page ``block_table[b, t // page_size]`` at place ``t % pa
 Handing out pages is the caller's: any order, pages shared between sequences (a common prompt) included, as long as no slot is
 written twice in one call.
 
-A layer's step for one new token a sequence is ``longctx.ops.rotary_``, ``paged_write``, ``attention.ops.paged_decode``; a later
-chunk of a prompt attends over ``paged_read`` rows with ``attention.ops.prefill_core``. Tables, lengths, slots and positions
+A layer's step for one new token a sequence is ``longctx.ops.rotary_``, ``paged_write``, ``attention.ops.paged_decode``. A later
+chunk of a prompt attends over ``paged_read`` rows with ``attention.ops.prefill_core``, one sequence a call: ``prefill_core`` has one
+position for its whole batch, and the zero rows that ``paged_read`` puts behind shorter sequences are keys like any others to it. Tables, lengths, slots and positions
 stay on the device and are read by the kernels alone, so the calls can be captured into a graph and replayed with others in
 their place (graphs that share a memory pool in the order of their capture, as torch asks for: a later one's tensors may lie where
 an earlier one had its workspace). There is no CPU path.
@@ -37,7 +38,7 @@ def paged_write(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
 def paged_read(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, length: int, head_size: Optional[int] = None,
                dtype: Optional[torch.dtype] = None, quant: Optional[ops.QuantState] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The first ``length`` rows of every sequence, ``(key, value)`` of shape (sequences, n_query_groups, length, head_size): rows behind
-    ``lens`` (int32, on the device) are zero. Pages of codes need ``quant``, and ``head_size`` and ``dtype`` of the rows
+    ``lens`` (int32, on the device) are zero (an attention that takes them for keys has to mask them). Pages of codes need ``quant``, and ``head_size`` and ``dtype`` of the rows
     they stand for; of plain pages both are known."""
     if quant is None:
         head_size = key_pages.shape[-1] if head_size is None else head_size
