@@ -552,6 +552,7 @@ int kvx_paged_read(const kvx_paged_read_args* args, void* stream);
  * log-sum-exp, fp32 (B, Hq) contiguous. q, o: (B, Hq, D) of the store's element type by strides; Hq / Hkv at most 16. Rows of codes stand for
  * (code - zp) * scale, not rounded to 16 bits in between. lens[b] is taken between 0 and max_pages * page_size; tokens in pages that the pool
  * does not have are left out. A sequence without tokens gets zeros and -inf. Rows behind lens[b] may hold anything, infinities and NaN included.
+ * A weight over codes is held with its row's scale, relative to the largest scale of the V rows before it: rows whose scale is below 2^-20 of that lose bits.
  * Weights count as positive, so that an infinite value of a row makes its output infinite; a row of codes whose scale is not finite makes its heads' outputs infinite or NaN.
  * The lengths are read on the device alone, so a captured call may be replayed with others. Work is dealt out to a fixed number of workgroups by the
  * lengths' sum, in shares of whole 128 tokens, whatever their distribution; results do not depend on anything but the arguments and that number.

@@ -26,8 +26,8 @@
 // 16 heads of 64 over 3000 to 50000 keys, 4-bit, fp16: 2.20e-4 off in the mean, and 2.04e-4, which is the rounding of the outputs, with the middle code taken off before
 // (16 sequences of 16384, 32 / 8 heads, 8-bit and 4-bit codes: rows of 64 +0 and 4 %, of 128 1 and 2 %, of 256 0 and 2 % longer).
 //
-// Bounds, 16 sequences of 16384 tokens, 32 / 8 heads: plain rows are at HBM (64 values 85 us, 128 158, 256 352: 6.3, 6.8, 6.1 TB/s), 8-bit rows of 128 too (91: 6.3). 8-bit
-// rows of 64 (53.6: 5.7) and 4-bit ones (64 values 42, 128 55, 256 95: 4.0, 5.5, 6.0) have as much to do in the vector ALU as in memory: per 32 keys of 64 4-bit
+// Bounds, 16 sequences of 16384 tokens, 32 / 8 heads: plain rows are at HBM (64 values 85 us, 128 158, 256 352: 6.3, 6.8, 6.1 TB/s), 8-bit rows of 128 nearly (91: 6.2). 8-bit
+// rows of 64 (53.6: 5.6) and 4-bit ones (64 values 42, 128 55, 256 95: 4.0, 5.5, 6.0) have as much to do in the vector ALU as in memory: per 32 keys of 64 4-bit
 // values some 230 vector instructions and 8 loads. Neither a third wavefront a SIMD nor a second block of keys in flight shortens them
 // by more than 3 %. A call's fixed part is 5 us of serial loads (lengths, table, rows) and a join of 3 to 5, most of it the launch.
 #include <type_traits>

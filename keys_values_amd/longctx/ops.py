@@ -125,6 +125,7 @@ def rotary_(qkv: torch.Tensor, n_head: int, n_query_groups: int, head_size: int,
 
     The tables' width says how much of a head is rotated: its first 2 * cos.shape[1] values (a multiple of 16). Pairs are the halves of that part, or with
     ``interleaved`` neighbours; frequencies for long contexts come with the tables (``rope_tables``). Tokens of a negative
-    position, and of one behind the tables, are left as they are. Returns qkv."""
+    position (padding), and of one behind the tables, are left as they are. The positions are read on the device alone, so nothing is raised for
+    those behind the tables: make the tables as long as the cache's sequences can get. Returns qkv."""
     _lib.host().rotary(qkv, n_head, n_query_groups, head_size, q_weight, k_weight, eps, cos, sin, positions, interleaved)
     return qkv
