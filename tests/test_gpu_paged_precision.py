@@ -131,3 +131,24 @@ def test_infinite_values_in_masked_places(gpu, store):
             pool.buffers.quant.v_scale[p, 0, places] = math.inf
     after = pool.buffers.decode(q, pool.table_gpu, pool.lens_gpu)[0]
     assert torch.isfinite(before).all() and torch.equal(before, after)
+
+
+@pytest.mark.parametrize("page", [16, 256])
+@pytest.mark.parametrize("store", ["bf16", "fp16"])
+def test_infinite_values_beside_masked_ones(gpu, store, page):
+    """The column of a live infinite value holds infinities of the other sign, and NaN, in masked places."""
+    pool = Pool(gpu, store, [3 * page + 5, 2 * page, 7], 2, 128, page, seed=6)
+    q = torch.randn(3, 8, 128, generator=pool.gen).to(pool.dtype).to(gpu)
+    v = pool.buffers.v
+    for b, n in enumerate(pool.lens):
+        v[int(pool.table[b, 0]), :, 4, 9] = math.inf
+        last = int(pool.table[b, (n - 1) // page])
+        v[last, :, (n - 1) % page + 1 :, 9] = -math.inf
+        v[last, :, (n - 1) % page + 1 :, 10] = math.nan
+    for b, at, entry in ((0, 1, -1), (1, 1, pool.num_pages + 7)):
+        v[int(pool.table[b, at]), :, :, 9] = math.nan
+        pool.table_gpu[b, at] = entry
+    out, lse = pool.buffers.decode(q, pool.table_gpu, pool.lens_gpu, return_lse=True)
+    assert torch.isfinite(lse).all() and (out[..., 9] == math.inf).all()
+    out[..., 9] = 0.0
+    assert torch.isfinite(out).all()
