@@ -575,6 +575,72 @@ typedef struct kvx_paged_decode_args {
 int kvx_paged_decode(const kvx_paged_decode_args* args, void* stream);
 size_t kvx_paged_decode_workspace_bytes(const kvx_paged_decode_args* args);
 
+/* ---- sparse attention over a paged cache: single tokens attend to the pages that their queries choose ---------------------- */
+
+/* What a layer writes for new tokens, in one call: kvx_rotary of the query heads, in place, and of the key heads on their way to their slots, which kvx_paged_write's of
+ * the value heads are too (rotary.qkv holds all of them; its key and value heads are left as they are). To the bit what the two calls store. A token whose
+ * position is negative or behind the tables' last row is padding: nothing of it is changed or stored, whatever its slot. One without a slot has its queries turned.
+ * Two tokens of one call with the same slot: one of them is stored, or parts of each. rotary's Hkv, D and elem_dtype have to fit the pages. A call takes fewer than
+ * 2^23 groups of 2048 / D heads: of tokens * Hq queries and tokens * Hkv plain rows, of codes Hkv times the groups of tokens. */
+typedef struct kvx_paged_append_args {
+  kvx_rotary_args rotary;
+  kvx_pages pages;
+  const int64_t* slots;
+} kvx_paged_append_args;
+int kvx_paged_append(const kvx_paged_append_args* args, void* stream);
+
+/* Bounds of keys. For the pages that hold the last `tokens` of the first lens[b] tokens of every sequence (the same for all; shorter sequences: all of their pages):
+ * the lowest and the highest of the page's keys among these lens[b], value by value, to bounds[page * b_stride_page + h * b_stride_h + d] and, b_stride_side further,
+ * of the store's element type. Rows of codes count as kvx_paged_read gives them. A NaN among a page's values makes its bounds NaN. Bounds of other pages, and of pages
+ * that the pool does not have, are left as they are. A page of two sequences gets the bounds of one of them: share pages that are full, or have as many tokens in
+ * both. pages.v and the state of V are not read, but checked. lens and the table are read on the device alone. A call looks at fewer than 2^22 (sequence,
+ * page, KV head), shorter sequences counted as the longest that the table and `tokens` allow. */
+typedef struct kvx_paged_bounds_args {
+  kvx_pages pages;
+  int32_t B, max_pages, tokens;
+  const int32_t* block_table; /* (B, max_pages) */
+  int64_t bt_stride_b;
+  const int32_t* lens; /* (B) */
+  void* bounds;
+  int64_t b_stride_page, b_stride_h, b_stride_side;
+} kvx_paged_bounds_args;
+int kvx_paged_bounds(const kvx_paged_bounds_args* args, void* stream);
+
+/* The pages that a query attends to. A page of a sequence (the i-th, i < ceil(lens[b] / page_size) and max_pages) has for KV head h the score
+ *   max over the query heads of h of sum_d max(q[d] * low[d], q[d] * high[d]),
+ * which is no less than any of its keys' products with them. Sums are formed in 64 bits and rounded to 32; a score that is not finite counts as infinite. Of every (sequence, KV head)
+ * the first `first` and the last `last` pages are chosen, and the others by their scores, of equal ones those in front: `count` pages, or all if there are no more. Pages that
+ * the pool does not have are not chosen. chosen: int32 (B, Hkv, count), contiguous: the pages' places in the table's row, rising, and -1 behind.
+ * first, last >= 0, first + last <= count. q, bounds: elem_dtype KVX_KV_BF16 / KVX_KV_F16; Hq / Hkv at most 16. workspace: kvx_paged_select_workspace_bytes(), contents do not
+ * matter; calls that may overlap need one each. */
+typedef struct kvx_paged_select_args {
+  int32_t num_pages, page_size, Hkv, D, elem_dtype, B, Hq, max_pages, count, first, last;
+  const void* q;
+  int64_t q_stride_b, q_stride_h;
+  const void* bounds; /* as kvx_paged_bounds_args has them */
+  int64_t b_stride_page, b_stride_h, b_stride_side;
+  const int32_t* block_table; /* (B, max_pages) */
+  int64_t bt_stride_b;
+  const int32_t* lens; /* (B) */
+  int32_t* chosen;
+  void* workspace;
+  size_t workspace_bytes;
+} kvx_paged_select_args;
+int kvx_paged_select(const kvx_paged_select_args* args, void* stream);
+size_t kvx_paged_select_workspace_bytes(const kvx_paged_select_args* args);
+
+/* kvx_paged_decode over some of a sequence's pages: those whose places in its table's row the list of a (sequence, KV head) names, int32 (B, Hkv, count) by strides, entries
+ * contiguous. As many of a list's entries are read as the sequence has pages, at most `count`. Entries that are negative or name no page with tokens are left out (also -1 behind shorter
+ * lists); any order; a page that is named twice counts twice. A pair without a token gets zeros and -inf. workspace:
+ * kvx_paged_decode_chosen_workspace_bytes(). */
+typedef struct kvx_chosen_pages {
+  const int32_t* pages;
+  int64_t stride_b, stride_h;
+  int32_t count;
+} kvx_chosen_pages;
+int kvx_paged_decode_chosen(const kvx_paged_decode_args* args, const kvx_chosen_pages* chosen, void* stream);
+size_t kvx_paged_decode_chosen_workspace_bytes(const kvx_paged_decode_args* args, const kvx_chosen_pages* chosen);
+
 #ifdef __cplusplus
 }
 #endif

@@ -167,6 +167,40 @@ class PagedDecodeArgs(ctypes.Structure):
     ]
 
 
+class PagedAppendArgs(ctypes.Structure):
+    """struct kvx_paged_append_args"""
+
+    _fields_ = [("rotary", RotaryArgs), ("pages", Pages), ("slots", c_void_p)]
+
+
+class PagedBoundsArgs(ctypes.Structure):
+    """struct kvx_paged_bounds_args"""
+
+    _fields_ = [
+        ("pages", Pages), ("B", c_int32), ("max_pages", c_int32), ("tokens", c_int32),
+        ("block_table", c_void_p), ("bt_stride_b", c_int64), ("lens", c_void_p),
+        ("bounds", c_void_p), ("b_stride_page", c_int64), ("b_stride_h", c_int64), ("b_stride_side", c_int64),
+    ]
+
+
+class PagedSelectArgs(ctypes.Structure):
+    """struct kvx_paged_select_args"""
+
+    _fields_ = [
+        *((name, c_int32) for name in ("num_pages", "page_size", "Hkv", "D", "elem_dtype", "B", "Hq", "max_pages", "count", "first", "last")),
+        ("q", c_void_p), ("q_stride_b", c_int64), ("q_stride_h", c_int64),
+        ("bounds", c_void_p), ("b_stride_page", c_int64), ("b_stride_h", c_int64), ("b_stride_side", c_int64),
+        ("block_table", c_void_p), ("bt_stride_b", c_int64), ("lens", c_void_p),
+        ("chosen", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class ChosenPages(ctypes.Structure):
+    """struct kvx_chosen_pages"""
+
+    _fields_ = [("pages", c_void_p), ("stride_b", c_int64), ("stride_h", c_int64), ("count", c_int32)]
+
+
 # every symbol include/kvx.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "kvx_version": (ctypes.c_int, []),
@@ -214,6 +248,12 @@ SYMBOLS = {
     "kvx_paged_read": (ctypes.c_int, [POINTER(PagedReadArgs), c_void_p]),
     "kvx_paged_decode": (ctypes.c_int, [POINTER(PagedDecodeArgs), c_void_p]),
     "kvx_paged_decode_workspace_bytes": (c_size_t, [POINTER(PagedDecodeArgs)]),
+    "kvx_paged_append": (ctypes.c_int, [POINTER(PagedAppendArgs), c_void_p]),
+    "kvx_paged_bounds": (ctypes.c_int, [POINTER(PagedBoundsArgs), c_void_p]),
+    "kvx_paged_select": (ctypes.c_int, [POINTER(PagedSelectArgs), c_void_p]),
+    "kvx_paged_select_workspace_bytes": (c_size_t, [POINTER(PagedSelectArgs)]),
+    "kvx_paged_decode_chosen": (ctypes.c_int, [POINTER(PagedDecodeArgs), POINTER(ChosenPages), c_void_p]),
+    "kvx_paged_decode_chosen_workspace_bytes": (c_size_t, [POINTER(PagedDecodeArgs), POINTER(ChosenPages)]),
 }
 
 _lib = None

@@ -5,6 +5,8 @@ from .ops import (  # noqa: F401
     get_load_error,
     is_available,
     paged_decode,
+    paged_decode_chosen,
+    paged_select,
     sdpa_decode,
     sdpa_prefill,
     sdpa_prefill_fused,

@@ -171,6 +171,39 @@ def paged_decode(
     return _lib.host().paged_decode(query, key_pages, value_pages, block_table, lens, scale, return_lse, quant)
 
 
+def paged_select(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, page_size: int, count: int, first: int = 1,
+                 last: int = 1) -> torch.Tensor:
+    """The pages that the new token of every sequence attends to: for each KV head the ``first`` and the ``last`` pages of the sequence and, up to ``count`` in
+    all, those whose keys' ``bounds`` (num_pages, n_query_groups, 2, head_size: see ``kvcache.paged.paged_bounds``) allow the largest product with one of the head's
+    queries,
+
+        max over the group's query heads of sum_d max(q[d] * lowest[d], q[d] * highest[d]),
+
+    of equal ones those in front. Sums are formed in 64 bits and rounded to 32, so that the choice does not depend on how the work is split; what is not finite counts
+    as infinite. query (B, Hq, D); ``block_table`` (B, max_pages) and ``lens`` (B,) as for :func:`paged_decode`. Returns int32 (B, Hkv, count): places in the
+    sequence's row of the table, rising, and -1 behind where it has fewer pages (all of them are chosen then). Pages that the pool does not have are
+    not chosen. ``last`` of 1 or more keeps the page that the new token has been written to."""
+    return _lib.host().paged_select(query, bounds, block_table, lens, page_size, count, first, last)
+
+
+def paged_decode_chosen(
+    query: torch.Tensor,
+    key_pages: torch.Tensor,
+    value_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    lens: torch.Tensor,
+    chosen: torch.Tensor,
+    scale: float,
+    return_lse: bool = False,
+    quant: Optional[QuantState] = None,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """:func:`paged_decode` over the rows of some pages alone: ``chosen`` int32 (B, Hkv, count) names, for each sequence and KV head, places in the sequence's
+    row of the table, as :func:`paged_select` returns them. As many entries of a list are read as the sequence has pages, ``count`` at most, in any order; entries that are
+    negative, or behind the sequence's last page, are left out, and a page that is named twice counts twice. The log-sum-exp is that of the chosen rows;
+    without any, the outputs are zeros and it is -inf. Several new tokens of a sequence: give its row of the table once for each, with lengths of their own."""
+    return _lib.host().paged_decode_chosen(query, key_pages, value_pages, block_table, lens, chosen, scale, return_lse, quant)
+
+
 # ---- the reference's entry points (keys_values/attention/flashinfer_ops.py:193-440) --------------
 
 

@@ -54,6 +54,12 @@ struct Lib {
   decltype(&::kvx_paged_read) kvx_paged_read = nullptr;
   decltype(&::kvx_paged_decode) kvx_paged_decode = nullptr;
   decltype(&::kvx_paged_decode_workspace_bytes) kvx_paged_decode_workspace_bytes = nullptr;
+  decltype(&::kvx_paged_append) kvx_paged_append = nullptr;
+  decltype(&::kvx_paged_bounds) kvx_paged_bounds = nullptr;
+  decltype(&::kvx_paged_select) kvx_paged_select = nullptr;
+  decltype(&::kvx_paged_select_workspace_bytes) kvx_paged_select_workspace_bytes = nullptr;
+  decltype(&::kvx_paged_decode_chosen) kvx_paged_decode_chosen = nullptr;
+  decltype(&::kvx_paged_decode_chosen_workspace_bytes) kvx_paged_decode_chosen_workspace_bytes = nullptr;
   bool bound = false;
 } lib;
 
@@ -943,10 +949,8 @@ PyObject* qk_norm_rope(PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
-// rotary(qkv, n_head, n_query_groups, head_size, q_weight or None, k_weight or None, eps, cos, sin, positions, interleaved)
-PyObject* rotary(PyObject* const* args, Py_ssize_t n) {
-  require_args(n, 11, "rotary");
-  require_entry(lib.kvx_rotary, "kvx_rotary");
+// args: qkv, n_head, n_query_groups, head_size, q_weight or None, k_weight or None, eps, cos, sin, positions; `interleaved`
+kvx_rotary_args rotary_args(PyObject* const* args, PyObject* interleaved) {
   const at::Tensor &qkv = tensor(args[0], "qkv"), &cos = tensor(args[7], "cos"), &sin = tensor(args[8], "sin"), &positions = tensor(args[9], "positions");
   const at::Tensor *qw = opt_tensor(args[4], "q_weight"), *kw = opt_tensor(args[5], "k_weight");
   require_together(qkv, {&cos, &sin, &positions, qw, kw});
@@ -987,7 +991,7 @@ PyObject* rotary(PyObject* const* args, Py_ssize_t n) {
   a.Hkv = (int32_t)hkv;
   a.D = (int32_t)d;
   a.rotary_dim = (int32_t)(2 * cos.size(1));
-  a.interleaved = truth(args[10]);
+  a.interleaved = truth(interleaved);
   a.elem_dtype = elem_dtype(type);
   a.table_rows = (int32_t)cos.size(0);
   a.eps = (float)real(args[6]);
@@ -996,6 +1000,15 @@ PyObject* rotary(PyObject* const* args, Py_ssize_t n) {
   a.cos = (const float*)cos.data_ptr();
   a.sin = (const float*)sin.data_ptr();
   a.positions = (const int32_t*)positions.data_ptr();
+  return a;
+}
+
+// rotary(qkv, n_head, n_query_groups, head_size, q_weight or None, k_weight or None, eps, cos, sin, positions, interleaved)
+PyObject* rotary(PyObject* const* args, Py_ssize_t n) {
+  require_args(n, 11, "rotary");
+  require_entry(lib.kvx_rotary, "kvx_rotary");
+  const kvx_rotary_args a = rotary_args(args, args[10]);
+  const at::Tensor& qkv = tensor(args[0], "qkv");
   const Launch L(qkv);
   check(unlocked([&] { return lib.kvx_rotary(&a, L.stream); }));
   Py_RETURN_NONE;
@@ -1143,14 +1156,10 @@ PyObject* paged_read(PyObject* const* args, Py_ssize_t n) {
   return two(key, value);
 }
 
-// paged_decode(query, key_pages, value_pages, block_table, lens, scale, return_lse, quant or None) -> (out (B, Hq, D), lse (B, Hq) or None)
-PyObject* paged_decode(PyObject* const* args, Py_ssize_t n) {
-  require_args(n, 8, "paged_decode");
-  require_entry(lib.kvx_paged_decode, "kvx_paged_decode");
+// A call's query, pages and sequences; args: query, key_pages, value_pages, block_table, lens
+kvx_paged_decode_args decode_args(PyObject* const* args, const std::optional<Quant>& qs) {
   const at::Tensor &q = tensor(args[0], "query"), &kp = tensor(args[1], "key_pages"), &vp = tensor(args[2], "value_pages"), &table = tensor(args[3], "block_table"),
                    &lens = tensor(args[4], "lens");
-  std::optional<Quant> qs;
-  if (args[7] != Py_None) qs.emplace(args[7]);
   require_together(q, {&kp, &vp, &table, &lens});
   require_state(q, qs);
   const at::ScalarType type = q.scalar_type();
@@ -1166,29 +1175,180 @@ PyObject* paged_decode(PyObject* const* args, Py_ssize_t n) {
   a.B = (int32_t)q.size(0);
   a.Hq = (int32_t)q.size(1);
   a.max_pages = (int32_t)table.size(1);
-  a.sm_scale = (float)real(args[5]);
   a.q = q.data_ptr();
   a.q_stride_b = q.size(0) > 1 ? q.stride(0) : 0;
   a.q_stride_h = q.size(1) > 1 ? q.stride(1) : 0;
   a.block_table = (const int32_t*)table.data_ptr();
   a.bt_stride_b = table.size(0) > 1 ? table.stride(0) : 0;
   a.lens = (const int32_t*)lens.data_ptr();
-  const bool want_lse = truth(args[6]);
+  return a;
+}
+// Outputs and workspace of a call, and its launch
+template <typename Bytes, typename Call>
+PyObject* decoded(kvx_paged_decode_args& a, const at::Tensor& q, bool want_lse, Bytes&& bytes, Call&& call) {
   const Launch L(q);
   at::Tensor out, lse;
   check(unlocked([&] {
-    out = L.empty({a.B, a.Hq, a.pages.D}, type);
+    out = L.empty({a.B, a.Hq, a.pages.D}, q.scalar_type());
     if (want_lse) lse = L.empty({a.B, a.Hq}, at::kFloat);
     a.o = out.data_ptr();
     a.o_stride_b = (int64_t)a.Hq * a.pages.D;
     a.o_stride_h = a.pages.D;
     a.lse = (float*)data(lse);
-    const at::Tensor ws = L.scratch(lib.kvx_paged_decode_workspace_bytes(&a));
+    const at::Tensor ws = L.scratch(bytes());
     a.workspace = data(ws);
     a.workspace_bytes = ws.defined() ? (size_t)ws.numel() : 0;
-    return lib.kvx_paged_decode(&a, L.stream);
+    return call(L.stream);
   }));
   return two(out, lse);
+}
+
+// paged_decode(query, key_pages, value_pages, block_table, lens, scale, return_lse, quant or None) -> (out (B, Hq, D), lse (B, Hq) or None)
+PyObject* paged_decode(PyObject* const* args, Py_ssize_t n) {
+  require_args(n, 8, "paged_decode");
+  require_entry(lib.kvx_paged_decode, "kvx_paged_decode");
+  std::optional<Quant> qs;
+  if (args[7] != Py_None) qs.emplace(args[7]);
+  kvx_paged_decode_args a = decode_args(args, qs);
+  a.sm_scale = (float)real(args[5]);
+  return decoded(a, tensor(args[0], "query"), truth(args[6]), [&] { return lib.kvx_paged_decode_workspace_bytes(&a); }, [&](void* stream) { return lib.kvx_paged_decode(&a, stream); });
+}
+
+// paged_decode_chosen(query, key_pages, value_pages, block_table, lens, chosen, scale, return_lse, quant or None) -> as paged_decode
+PyObject* paged_decode_chosen(PyObject* const* args, Py_ssize_t n) {
+  require_args(n, 9, "paged_decode_chosen");
+  require_entry(lib.kvx_paged_decode_chosen, "kvx_paged_decode_chosen");
+  std::optional<Quant> qs;
+  if (args[8] != Py_None) qs.emplace(args[8]);
+  const at::Tensor &q = tensor(args[0], "query"), &chosen = tensor(args[5], "chosen");
+  require_together(q, {&chosen});
+  kvx_paged_decode_args a = decode_args(args, qs);
+  a.sm_scale = (float)real(args[6]);
+  if (chosen.scalar_type() != at::kInt || chosen.dim() != 3 || chosen.size(0) != a.B || chosen.size(1) != a.pages.Hkv || chosen.size(2) == 0 || chosen.size(2) > INT32_MAX ||
+      chosen.stride(2) != 1)
+    raise(PyExc_ValueError, "chosen must be an int32 (%d, %d, pages) tensor with a contiguous last axis, got %s of shape %s", a.B, a.pages.Hkv,
+          dtype_name(chosen.scalar_type()).c_str(), shape_str(chosen).c_str());
+  const kvx_chosen_pages c = {(const int32_t*)chosen.data_ptr(), chosen.stride(0), chosen.stride(1), (int32_t)chosen.size(2)};
+  return decoded(a, q, truth(args[7]), [&] { return lib.kvx_paged_decode_chosen_workspace_bytes(&a, &c); },
+                 [&](void* stream) { return lib.kvx_paged_decode_chosen(&a, &c, stream); });
+}
+
+// paged_append(qkv, n_head, n_query_groups, head_size, q_weight or None, k_weight or None, eps, cos, sin, positions, key_pages, value_pages, slots, quant or None, interleaved)
+PyObject* paged_append(PyObject* const* args, Py_ssize_t n) {
+  require_args(n, 15, "paged_append");
+  require_entry(lib.kvx_paged_append, "kvx_paged_append");
+  const at::Tensor &qkv = tensor(args[0], "qkv"), &kp = tensor(args[10], "key_pages"), &vp = tensor(args[11], "value_pages"), &slots = tensor(args[12], "slots");
+  std::optional<Quant> qs;
+  if (args[13] != Py_None) qs.emplace(args[13]);
+  require_together(qkv, {&kp, &vp, &slots});
+  require_state(qkv, qs);
+  kvx_paged_append_args a{};
+  a.rotary = rotary_args(args, args[14]);
+  a.pages = pages_of(kp, vp, qs ? &*qs : nullptr, a.rotary.D, qkv.scalar_type());
+  if (a.pages.Hkv != a.rotary.Hkv) raise(PyExc_ValueError, "n_query_groups = %d does not fit pages of %d heads", a.rotary.Hkv, a.pages.Hkv);
+  if (slots.scalar_type() != at::kLong || slots.numel() != a.rotary.tokens || !slots.is_contiguous())
+    raise(PyExc_ValueError, "slots must be a contiguous int64 tensor of %lld tokens, got %s of shape %s", (long long)a.rotary.tokens, dtype_name(slots.scalar_type()).c_str(),
+          shape_str(slots).c_str());
+  a.slots = (const int64_t*)slots.data_ptr();
+  const Launch L(qkv);
+  check(unlocked([&] { return lib.kvx_paged_append(&a, L.stream); }));
+  Py_RETURN_NONE;
+}
+
+// bounds (num_pages, n_query_groups, 2, head_size) with contiguous rows
+void check_bounds(const at::Tensor& bounds) {
+  const at::ScalarType type = bounds.scalar_type();
+  if (type != at::kBFloat16 && type != at::kHalf)
+    raise(PyExc_NotImplementedError, "bounds.dtype must be torch.bfloat16 or torch.float16, got %s", dtype_name(type).c_str());
+  if (bounds.dim() != 4 || bounds.size(2) != 2 || bounds.stride(3) != 1 || bounds.size(0) == 0 || bounds.size(0) > INT32_MAX || bounds.size(1) == 0 || bounds.size(1) > INT32_MAX)
+    raise(PyExc_ValueError, "bounds must be (num_pages, n_query_groups, 2, head_size) with contiguous rows, got shape %s", shape_str(bounds).c_str());
+  check_head_size(bounds.size(3));
+}
+
+// paged_bounds(key_pages, bounds, block_table, lens, tokens or None, quant or None)
+PyObject* paged_bounds(PyObject* const* args, Py_ssize_t n) {
+  require_args(n, 6, "paged_bounds");
+  require_entry(lib.kvx_paged_bounds, "kvx_paged_bounds");
+  const at::Tensor &kp = tensor(args[0], "key_pages"), &bounds = tensor(args[1], "bounds"), &table = tensor(args[2], "block_table"), &lens = tensor(args[3], "lens");
+  std::optional<Quant> qs;
+  if (args[5] != Py_None) qs.emplace(args[5]);
+  require_together(kp, {&bounds, &table, &lens});
+  require_state(kp, qs);
+  check_bounds(bounds);
+  kvx_paged_bounds_args a{};
+  a.pages = pages_of(kp, kp, qs ? &*qs : nullptr, bounds.size(3), bounds.scalar_type());
+  if (bounds.size(0) != a.pages.num_pages || bounds.size(1) != a.pages.Hkv)
+    raise(PyExc_ValueError, "bounds of shape %s do not fit pages of shape %s", shape_str(bounds).c_str(), shape_str(kp).c_str());
+  check_sequences(table, lens);
+  const int64_t all = std::min((int64_t)INT32_MAX, table.size(1) * a.pages.page_size), tokens = args[4] == Py_None ? all : integer(args[4]);
+  if (tokens < 0) raise(PyExc_ValueError, "tokens = %lld", (long long)tokens);
+  a.B = (int32_t)table.size(0);
+  a.max_pages = (int32_t)table.size(1);
+  a.tokens = (int32_t)std::min(tokens, all);
+  a.block_table = (const int32_t*)table.data_ptr();
+  a.bt_stride_b = table.size(0) > 1 ? table.stride(0) : 0;
+  a.lens = (const int32_t*)lens.data_ptr();
+  a.bounds = bounds.data_ptr();
+  a.b_stride_page = bounds.stride(0);
+  a.b_stride_h = bounds.stride(1);
+  a.b_stride_side = bounds.stride(2);
+  const Launch L(kp);
+  check(unlocked([&] { return lib.kvx_paged_bounds(&a, L.stream); }));
+  Py_RETURN_NONE;
+}
+
+// paged_select(query, bounds, block_table, lens, page_size, count, first, last) -> chosen (B, Hkv, count) int32
+PyObject* paged_select(PyObject* const* args, Py_ssize_t n) {
+  require_args(n, 8, "paged_select");
+  require_entry(lib.kvx_paged_select, "kvx_paged_select");
+  const at::Tensor &q = tensor(args[0], "query"), &bounds = tensor(args[1], "bounds"), &table = tensor(args[2], "block_table"), &lens = tensor(args[3], "lens");
+  require_together(q, {&bounds, &table, &lens});
+  check_bounds(bounds);
+  if (q.scalar_type() != bounds.scalar_type())
+    raise(PyExc_NotImplementedError, "query.dtype must be that of the bounds, %s, got %s", dtype_name(bounds.scalar_type()).c_str(), dtype_name(q.scalar_type()).c_str());
+  if (q.dim() != 3 || q.stride(2) != 1 || q.size(2) != bounds.size(3))
+    raise(PyExc_ValueError, "query must be (sequences, n_head, %lld) with contiguous rows, got shape %s", (long long)bounds.size(3), shape_str(q).c_str());
+  check_heads(q.size(1), bounds.size(1));
+  check_sequences(table, lens);
+  if (table.size(0) != q.size(0)) raise(PyExc_ValueError, "block_table has %lld rows for %lld sequences", (long long)table.size(0), (long long)q.size(0));
+  int64_t numbers[4];
+  for (int i = 0; i < 4; ++i) {
+    numbers[i] = integer(args[4 + i]);
+    if (numbers[i] < 0 || numbers[i] > INT32_MAX) raise(PyExc_ValueError, "%s = %lld", (const char*[]){"page_size", "count", "first", "last"}[i], (long long)numbers[i]);
+  }
+  kvx_paged_select_args a{};
+  a.num_pages = (int32_t)bounds.size(0);
+  a.Hkv = (int32_t)bounds.size(1);
+  a.D = (int32_t)bounds.size(3);
+  a.elem_dtype = elem_dtype(q.scalar_type());
+  a.page_size = (int32_t)numbers[0];
+  a.count = (int32_t)numbers[1];
+  a.first = (int32_t)numbers[2];
+  a.last = (int32_t)numbers[3];
+  a.B = (int32_t)q.size(0);
+  a.Hq = (int32_t)q.size(1);
+  a.max_pages = (int32_t)table.size(1);
+  a.q = q.data_ptr();
+  a.q_stride_b = q.size(0) > 1 ? q.stride(0) : 0;
+  a.q_stride_h = q.size(1) > 1 ? q.stride(1) : 0;
+  a.bounds = bounds.data_ptr();
+  a.b_stride_page = bounds.stride(0);
+  a.b_stride_h = bounds.stride(1);
+  a.b_stride_side = bounds.stride(2);
+  a.block_table = (const int32_t*)table.data_ptr();
+  a.bt_stride_b = table.size(0) > 1 ? table.stride(0) : 0;
+  a.lens = (const int32_t*)lens.data_ptr();
+  const Launch L(q);
+  at::Tensor chosen;
+  check(unlocked([&] {
+    chosen = L.empty({a.B, a.Hkv, a.count}, at::kInt);
+    a.chosen = (int32_t*)chosen.data_ptr();
+    const at::Tensor ws = L.scratch(lib.kvx_paged_select_workspace_bytes(&a));
+    a.workspace = data(ws);
+    a.workspace_bytes = ws.defined() ? (size_t)ws.numel() : 0;
+    return lib.kvx_paged_select(&a, L.stream);
+  }));
+  return wrap(chosen);
 }
 
 // ---- module -------------------------------------------------------------------------------------------------------------------
@@ -1210,6 +1370,7 @@ PyObject* bind(PyObject* const* args, Py_ssize_t n) {
   l.kvx_sdpa_prefill_first = (decltype(l.kvx_sdpa_prefill_first))dlsym(h, "kvx_sdpa_prefill_first");
 #define X(name) l.name = (decltype(l.name))dlsym(h, #name);
   X(kvx_rotary) X(kvx_paged_write) X(kvx_paged_read) X(kvx_paged_decode) X(kvx_paged_decode_workspace_bytes)
+  X(kvx_paged_append) X(kvx_paged_bounds) X(kvx_paged_select) X(kvx_paged_select_workspace_bytes) X(kvx_paged_decode_chosen) X(kvx_paged_decode_chosen_workspace_bytes)
 #undef X
   l.bound = true;
   lib = l;
@@ -1239,7 +1400,8 @@ PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void (*)(void))entry<bind, false>, METH_FASTCALL, nullptr},
     METHOD(prefill), METHOD(score_sum), METHOD(decode), METHOD(check_qkv), METHOD(cache_write), METHOD(cache_write_first), METHOD(prefill_first), METHOD(cache_update), METHOD(cache_decode_step),
     METHOD(quantize_blocks), METHOD(dequantize_blocks), METHOD(dequantize_rows), METHOD(rmsnorm), METHOD(add_rmsnorm),
-    METHOD(swiglu), METHOD(qk_norm_rope), METHOD(rotary), METHOD(paged_write), METHOD(paged_read), METHOD(paged_decode), {nullptr, nullptr, 0, nullptr}};
+    METHOD(swiglu), METHOD(qk_norm_rope), METHOD(rotary), METHOD(paged_write), METHOD(paged_read), METHOD(paged_decode), METHOD(paged_append), METHOD(paged_bounds),
+    METHOD(paged_select), METHOD(paged_decode_chosen), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "Native host path of the kernels (see csrc/host.cpp).", -1, methods};
 
 }  // namespace

@@ -478,23 +478,29 @@ int kvx_qk_norm_rope(void* qkv, int64_t stride_b, int64_t stride_t, int32_t B, i
   return launch_qk_norm_rope(qkv, stride_b, stride_t, B, num, Hq, Hkv, D, q_weight, k_weight, eps, cos, sin, input_pos, (hipStream_t)stream);
 }
 
-int kvx_rotary(const kvx_rotary_args* a, void* stream) {
-  KVX_REQUIRE(a != nullptr, KVX_ERR_INVALID, "kvx_rotary: args is NULL");
-  KVX_REQUIRE(a->tokens >= 0 && a->Hq > 0 && a->Hkv > 0, KVX_ERR_INVALID, "kvx_rotary: tokens=%lld Hq=%d Hkv=%d", (long long)a->tokens, a->Hq, a->Hkv);
-  KVX_REQUIRE(a->D == 64 || a->D == 128 || a->D == 256, KVX_ERR_UNSUPPORTED, "kvx_rotary: head size %d not in {64, 128, 256}", a->D);
-  KVX_REQUIRE(a->elem_dtype == KVX_KV_BF16 || a->elem_dtype == KVX_KV_F16, KVX_ERR_UNSUPPORTED, "kvx_rotary: unknown elem_dtype %d", a->elem_dtype);
+static int check_rotary(const kvx_rotary_args* a, const char* who) {
+  KVX_REQUIRE(a != nullptr, KVX_ERR_INVALID, "%s: args is NULL", who);
+  KVX_REQUIRE(a->tokens >= 0 && a->Hq > 0 && a->Hkv > 0, KVX_ERR_INVALID, "%s: tokens=%lld Hq=%d Hkv=%d", who, (long long)a->tokens, a->Hq, a->Hkv);
+  KVX_REQUIRE(a->D == 64 || a->D == 128 || a->D == 256, KVX_ERR_UNSUPPORTED, "%s: head size %d not in {64, 128, 256}", who, a->D);
+  KVX_REQUIRE(a->elem_dtype == KVX_KV_BF16 || a->elem_dtype == KVX_KV_F16, KVX_ERR_UNSUPPORTED, "%s: unknown elem_dtype %d", who, a->elem_dtype);
   KVX_REQUIRE(a->rotary_dim > 0 && a->rotary_dim <= a->D && a->rotary_dim % 16 == 0, KVX_ERR_UNSUPPORTED,
-              "kvx_rotary: rotary_dim=%d must be a multiple of 16, at most the head size %d", a->rotary_dim, a->D);
-  KVX_REQUIRE(a->Hq <= 65535 && a->Hkv <= 65535 && a->tokens <= INT32_MAX, KVX_ERR_UNSUPPORTED, "kvx_rotary: %lld tokens of %d + %d heads", (long long)a->tokens,
+              "%s: rotary_dim=%d must be a multiple of 16, at most the head size %d", who, a->rotary_dim, a->D);
+  KVX_REQUIRE(a->Hq <= 65535 && a->Hkv <= 65535 && a->tokens <= INT32_MAX, KVX_ERR_UNSUPPORTED, "%s: %lld tokens of %d + %d heads", who, (long long)a->tokens,
               a->Hq, a->Hkv);
-  KVX_REQUIRE(a->table_rows > 0, KVX_ERR_INVALID, "kvx_rotary: table_rows=%d", a->table_rows);
+  KVX_REQUIRE(a->table_rows > 0, KVX_ERR_INVALID, "%s: table_rows=%d", who, a->table_rows);
   if (a->tokens == 0) return KVX_OK;
-  KVX_REQUIRE(a->qkv && a->cos && a->sin && a->positions, KVX_ERR_INVALID, "kvx_rotary: NULL pointer");
-  KVX_REQUIRE((a->q_weight == nullptr) == (a->k_weight == nullptr), KVX_ERR_INVALID, "kvx_rotary: give both norm weights or none");
-  KVX_REQUIRE(a->tokens == 1 || a->stride_t >= ((int64_t)a->Hq + a->Hkv) * a->D, KVX_ERR_INVALID, "kvx_rotary: token stride %lld shorter than the query and key heads",
+  KVX_REQUIRE(a->qkv && a->cos && a->sin && a->positions, KVX_ERR_INVALID, "%s: NULL pointer", who);
+  KVX_REQUIRE((a->q_weight == nullptr) == (a->k_weight == nullptr), KVX_ERR_INVALID, "%s: give both norm weights or none", who);
+  KVX_REQUIRE(a->tokens == 1 || a->stride_t >= ((int64_t)a->Hq + a->Hkv) * a->D, KVX_ERR_INVALID, "%s: token stride %lld shorter than the query and key heads", who,
               (long long)a->stride_t);
   KVX_REQUIRE(aligned16(a->qkv) && aligned16(a->cos) && aligned16(a->sin) && mult8(a->stride_t) && (!a->q_weight || (aligned16(a->q_weight) && aligned16(a->k_weight))),
-              KVX_ERR_INVALID, "kvx_rotary: pointers and the token stride must keep 16-byte alignment");
+              KVX_ERR_INVALID, "%s: pointers and the token stride must keep 16-byte alignment", who);
+  return KVX_OK;
+}
+
+int kvx_rotary(const kvx_rotary_args* a, void* stream) {
+  const int rc = check_rotary(a, "kvx_rotary");
+  if (rc != KVX_OK || a->tokens == 0) return rc;
   return launch_rotary(*a, (hipStream_t)stream);
 }
 
@@ -574,8 +580,7 @@ int kvx_paged_read(const kvx_paged_read_args* a, void* stream) {
   return launch_paged_read(*a, (hipStream_t)stream);
 }
 
-static int check_paged_decode(const kvx_paged_decode_args* a) {
-  static const char who[] = "kvx_paged_decode";
+static int check_paged_decode(const kvx_paged_decode_args* a, const char* who) {
   KVX_REQUIRE(a != nullptr, KVX_ERR_INVALID, "%s: args is NULL", who);
   int rc = check_pages(a->pages, who);
   if (rc != KVX_OK) return rc;
@@ -591,21 +596,114 @@ static int check_paged_decode(const kvx_paged_decode_args* a) {
   return KVX_OK;
 }
 
+static int paged_decode(const kvx_paged_decode_args& a, const kvx_chosen_pages* chosen, const char* who, void* stream) {
+  int rc;
+  if (a.B == 0) return KVX_OK;
+  if ((rc = check_rows(a.q, "q", who, {a.q_stride_b, a.q_stride_h})) != KVX_OK) return rc;
+  if ((rc = check_rows(a.o, "o", who, {a.o_stride_b, a.o_stride_h})) != KVX_OK) return rc;
+  const size_t need = paged_decode_workspace(a, chosen);
+  KVX_REQUIRE(need == 0 || (aligned16(a.workspace) && a.workspace && a.workspace_bytes >= need), KVX_ERR_WORKSPACE,
+              "%s: workspace of %zu bytes, 16-byte aligned, is needed, got %zu", who, need, a.workspace ? a.workspace_bytes : (size_t)0);
+  return launch_paged_decode(a, chosen, (hipStream_t)stream);
+}
+
 int kvx_paged_decode(const kvx_paged_decode_args* a, void* stream) {
-  int rc = check_paged_decode(a);
-  if (rc != KVX_OK) return rc;
-  if (a->B == 0) return KVX_OK;
-  if ((rc = check_rows(a->q, "q", "kvx_paged_decode", {a->q_stride_b, a->q_stride_h})) != KVX_OK) return rc;
-  if ((rc = check_rows(a->o, "o", "kvx_paged_decode", {a->o_stride_b, a->o_stride_h})) != KVX_OK) return rc;
-  const size_t need = paged_decode_workspace(*a);
-  KVX_REQUIRE(need == 0 || (aligned16(a->workspace) && a->workspace && a->workspace_bytes >= need), KVX_ERR_WORKSPACE,
-              "kvx_paged_decode: workspace of %zu bytes, 16-byte aligned, is needed, got %zu", need, a->workspace ? a->workspace_bytes : (size_t)0);
-  return launch_paged_decode(*a, (hipStream_t)stream);
+  const int rc = check_paged_decode(a, "kvx_paged_decode");
+  return rc != KVX_OK ? rc : paged_decode(*a, nullptr, "kvx_paged_decode", stream);
 }
 
 size_t kvx_paged_decode_workspace_bytes(const kvx_paged_decode_args* a) {
-  if (check_paged_decode(a) != KVX_OK || a->B == 0) return 0;
-  return paged_decode_workspace(*a);
+  if (check_paged_decode(a, "kvx_paged_decode") != KVX_OK || a->B == 0) return 0;
+  return paged_decode_workspace(*a, nullptr);
+}
+
+// ---- sparse attention over a paged cache -----------------------------------------------------------------------------------------
+
+static int check_chosen(const kvx_paged_decode_args* a, const kvx_chosen_pages* c) {
+  static const char who[] = "kvx_paged_decode_chosen";
+  const int rc = check_paged_decode(a, who);
+  if (rc != KVX_OK) return rc;
+  KVX_REQUIRE(c != nullptr && c->count > 0, KVX_ERR_INVALID, "%s: a list of %d pages", who, c ? c->count : 0);
+  KVX_REQUIRE(a->B == 0 || (c->pages && c->stride_b >= 0 && c->stride_h >= 0), KVX_ERR_INVALID, "%s: the lists of pages must be given", who);
+  return KVX_OK;
+}
+
+int kvx_paged_decode_chosen(const kvx_paged_decode_args* a, const kvx_chosen_pages* c, void* stream) {
+  const int rc = check_chosen(a, c);
+  return rc != KVX_OK ? rc : paged_decode(*a, c, "kvx_paged_decode_chosen", stream);
+}
+
+size_t kvx_paged_decode_chosen_workspace_bytes(const kvx_paged_decode_args* a, const kvx_chosen_pages* c) {
+  if (check_chosen(a, c) != KVX_OK || a->B == 0) return 0;
+  return paged_decode_workspace(*a, c);
+}
+
+int kvx_paged_append(const kvx_paged_append_args* a, void* stream) {
+  static const char who[] = "kvx_paged_append";
+  int rc = check_rotary(a ? &a->rotary : nullptr, who);
+  if (rc != KVX_OK || (rc = check_pages(a->pages, who)) != KVX_OK) return rc;
+  const kvx_rotary_args& r = a->rotary;
+  KVX_REQUIRE(r.Hkv == a->pages.Hkv && r.D == a->pages.D && (r.elem_dtype == KVX_KV_F16) == kv_elem_f16(a->pages.kv_dtype), KVX_ERR_INVALID,
+              "%s: %d heads of %d, elem_dtype %d, do not fit pages of %d heads of %d, kv_dtype %d", who, r.Hkv, r.D, r.elem_dtype, a->pages.Hkv, a->pages.D, a->pages.kv_dtype);
+  if (r.tokens == 0) return KVX_OK;
+  KVX_REQUIRE(r.tokens == 1 || r.stride_t >= ((int64_t)r.Hq + 2 * (int64_t)r.Hkv) * r.D, KVX_ERR_INVALID, "%s: token stride %lld shorter than the heads", who, (long long)r.stride_t);
+  KVX_REQUIRE(a->slots, KVX_ERR_INVALID, "%s: slots must be given", who);
+  return launch_paged_append(*a, (hipStream_t)stream);
+}
+
+static int check_bounds(const void* bounds, int64_t stride_page, int64_t stride_h, int64_t stride_side, const char* who) {
+  int rc = check_rows(bounds, "bounds", who, {stride_page, stride_h, stride_side});
+  if (rc != KVX_OK) return rc;
+  KVX_REQUIRE(stride_page >= 0 && stride_h >= 0 && stride_side >= 0, KVX_ERR_INVALID, "%s: negative strides of the bounds", who);
+  return KVX_OK;
+}
+
+int kvx_paged_bounds(const kvx_paged_bounds_args* a, void* stream) {
+  static const char who[] = "kvx_paged_bounds";
+  KVX_REQUIRE(a != nullptr, KVX_ERR_INVALID, "%s: args is NULL", who);
+  int rc = check_pages(a->pages, who);
+  if (rc != KVX_OK) return rc;
+  if ((rc = check_sequences(who, a->B, a->max_pages, a->block_table, a->bt_stride_b, a->lens, a->pages.page_size)) != KVX_OK) return rc;
+  KVX_REQUIRE(a->tokens >= 0, KVX_ERR_INVALID, "%s: tokens=%d", who, a->tokens);
+  if (a->B == 0 || a->tokens == 0) return KVX_OK;
+  if ((rc = check_bounds(a->bounds, a->b_stride_page, a->b_stride_h, a->b_stride_side, who)) != KVX_OK) return rc;
+  return launch_paged_bounds(*a, (hipStream_t)stream);
+}
+
+static int check_select(const kvx_paged_select_args* a) {
+  static const char who[] = "kvx_paged_select";
+  KVX_REQUIRE(a != nullptr, KVX_ERR_INVALID, "%s: args is NULL", who);
+  KVX_REQUIRE(a->num_pages > 0 && a->Hkv > 0, KVX_ERR_INVALID, "%s: num_pages=%d Hkv=%d must be positive", who, a->num_pages, a->Hkv);
+  KVX_REQUIRE(a->page_size >= 16 && a->page_size <= 1024 && (a->page_size & (a->page_size - 1)) == 0, KVX_ERR_UNSUPPORTED,
+              "%s: page_size=%d must be a power of two from 16 to 1024", who, a->page_size);
+  KVX_REQUIRE(a->D == 64 || a->D == 128 || a->D == 256, KVX_ERR_UNSUPPORTED, "%s: head size %d not in {64, 128, 256}", who, a->D);
+  KVX_REQUIRE(a->elem_dtype == KVX_KV_BF16 || a->elem_dtype == KVX_KV_F16, KVX_ERR_UNSUPPORTED, "%s: unknown elem_dtype %d", who, a->elem_dtype);
+  int rc = check_sequences(who, a->B, a->max_pages, a->block_table, a->bt_stride_b, a->lens, a->page_size);
+  if (rc != KVX_OK) return rc;
+  KVX_REQUIRE(a->Hkv <= 65535, KVX_ERR_UNSUPPORTED, "%s: Hkv=%d beyond 65535", who, a->Hkv);
+  KVX_REQUIRE(a->Hq > 0 && a->Hq % a->Hkv == 0, KVX_ERR_INVALID, "%s: Hq=%d must be a positive multiple of Hkv=%d", who, a->Hq, a->Hkv);
+  KVX_REQUIRE(a->Hq / a->Hkv <= 16, KVX_ERR_UNSUPPORTED, "%s: %d query heads per KV head (at most 16)", who, a->Hq / a->Hkv);
+  KVX_REQUIRE(a->count > 0 && a->first >= 0 && a->last >= 0 && (int64_t)a->first + a->last <= a->count, KVX_ERR_INVALID,
+              "%s: count=%d must be positive, and first=%d and last=%d not negative and no more together", who, a->count, a->first, a->last);
+  return KVX_OK;
+}
+
+int kvx_paged_select(const kvx_paged_select_args* a, void* stream) {
+  static const char who[] = "kvx_paged_select";
+  int rc = check_select(a);
+  if (rc != KVX_OK || a->B == 0) return rc;
+  if ((rc = check_rows(a->q, "q", who, {a->q_stride_b, a->q_stride_h})) != KVX_OK) return rc;
+  if ((rc = check_bounds(a->bounds, a->b_stride_page, a->b_stride_h, a->b_stride_side, who)) != KVX_OK) return rc;
+  KVX_REQUIRE(a->chosen, KVX_ERR_INVALID, "%s: chosen must be given", who);
+  const size_t need = paged_select_workspace(*a);
+  KVX_REQUIRE(need == 0 || (aligned16(a->workspace) && a->workspace && a->workspace_bytes >= need), KVX_ERR_WORKSPACE,
+              "%s: workspace of %zu bytes, 16-byte aligned, is needed, got %zu", who, need, a->workspace ? a->workspace_bytes : (size_t)0);
+  return launch_paged_select(*a, (hipStream_t)stream);
+}
+
+size_t kvx_paged_select_workspace_bytes(const kvx_paged_select_args* a) {
+  if (check_select(a) != KVX_OK || a->B == 0) return 0;
+  return paged_select_workspace(*a);
 }
 
 }  // extern "C"

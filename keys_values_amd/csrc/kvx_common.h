@@ -114,8 +114,13 @@ int launch_qk_norm_rope(void* qkv, int64_t sb, int64_t stt, int B, int num, int 
 int launch_rotary(const kvx_rotary_args& a, hipStream_t st);
 int launch_paged_write(const kvx_paged_write_args& a, hipStream_t st);
 int launch_paged_read(const kvx_paged_read_args& a, hipStream_t st);
-int launch_paged_decode(const kvx_paged_decode_args& a, hipStream_t st);
-size_t paged_decode_workspace(const kvx_paged_decode_args& a);
+// chosen: the pages that are attended to, or NULL: all
+int launch_paged_decode(const kvx_paged_decode_args& a, const kvx_chosen_pages* chosen, hipStream_t st);
+size_t paged_decode_workspace(const kvx_paged_decode_args& a, const kvx_chosen_pages* chosen);
+int launch_paged_append(const kvx_paged_append_args& a, hipStream_t st);
+int launch_paged_bounds(const kvx_paged_bounds_args& a, hipStream_t st);
+int launch_paged_select(const kvx_paged_select_args& a, hipStream_t st);
+size_t paged_select_workspace(const kvx_paged_select_args& a);
 
 // Number of compute units of the current device (cached).
 int num_cus();

@@ -65,8 +65,22 @@ struct PagedParams {
   int* part_of;    // by pairs: the workgroup that left a pair's first partial; by workgroups: the pair; and how many partials the pair has, 0: none. NULL: no partials
 };
 
-// Units of a pair of `len` tokens: those with keys, and, behind them, as many without as the change to the pair takes the time of.
-__device__ __forceinline__ int units_of(int len, const PagedParams& p, int extra) { return max(1, (min(max(len, 0), p.cap) + (1 << p.unit) - 1) >> p.unit) + extra; }
+// Attention over chosen pages: entries (B, Hkv, count) by strides, of which a sequence has as many as pages, at most `count`; cap is that of the entries.
+struct ChosenParams : PagedParams {
+  const int* chosen;
+  int64_t ch_sb, ch_sh;
+  int table_cap;  // tokens of a table's pages
+};
+
+// Keys that a pair of a sequence of `len` tokens goes through: its tokens, or the places of the pages that are chosen
+template <typename Params>
+__device__ __forceinline__ int keys_of(int len, const Params& p) {
+  if constexpr (std::is_same_v<Params, ChosenParams>) return min((min(max(len, 0), p.table_cap) + (1 << p.shift) - 1) >> p.shift << p.shift, p.cap);
+  else return min(max(len, 0), p.cap);
+}
+// Units of a pair of a sequence of `len` tokens: those with keys, and, behind them, as many without as the change to the pair takes the time of.
+template <typename Params>
+__device__ __forceinline__ int units_of(int len, const Params& p, int extra) { return max(1, (keys_of(len, p) + (1 << p.unit) - 1) >> p.unit) + extra; }
 
 // Inclusive sum over the lanes of a wavefront, on the vector ALU.
 __device__ __forceinline__ int scan(int x) {
@@ -234,8 +248,10 @@ __device__ __forceinline__ T once(const void* p) { return __builtin_nontemporal_
 // asked to, which short pairs gain from (256 sequences of 50 to 400 tokens, 32 / 8 heads: 49.1 us with two, 42.8 with three). No bound here spills.
 constexpr int waves_per_simd(int D, bool codes) { return D == 256 && !codes ? 1 : D == 128 && !codes ? 3 : 2; }
 
-template <int D, int KV>
-__global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged_decode_kernel(const PagedParams p) {
+// CHOSEN: over the pages that a list names, of a (sequence, KV head) its own. A key's place in the pair is that in the list's pages then, one behind the other, and its place
+// in the sequence, which says whether there is such a token, comes of the list's entry: 16 keys are in one page, and `live` of them are tokens.
+template <int D, int KV, bool CHOSEN>
+__global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged_decode_kernel(const std::conditional_t<CHOSEN, ChosenParams, PagedParams> p) {
   using R = Rows<D, KV>;
   constexpr bool F16 = R::F16, CODES = R::CODES, U4 = R::U4, P16 = F16 || CODES;  // P16: weights and operands in fp16
   constexpr int KJ = R::KJ, DPL = R::DPL, ES = R::ES;
@@ -291,7 +307,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
 
   // A stretch of a pair's units. The next one's first rows are on their way while this one's results are joined.
   struct Stretch {
-    int b, h, begin, units, first, n, k_begin, k_end;
+    int b, h, begin, units, first, n, k_begin, k_end, tokens /* CHOSEN: of the sequence */;
   };
   auto go_to = [&](int to, int units) {  // to a unit of the same pair, or the next one's first
     unit = to;
@@ -308,15 +324,16 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
   }
   auto take = [&] {
     Stretch s;
-    const int len = min(max(__builtin_amdgcn_readlane(lane_len, b & 63), 0), p.cap);
+    const int len = __builtin_amdgcn_readlane(lane_len, b & 63);
     s.b = b;
+    if constexpr (CHOSEN) s.tokens = min(max(len, 0), p.table_cap);
     s.units = units_of(len, p, extra);
     s.h = (unit - begin_b) / s.units;
     s.begin = begin_b + s.h * s.units;
     s.first = unit - s.begin;
     s.n = min(s.units - s.first, end - unit);
     s.k_begin = s.first << p.unit;
-    s.k_end = min(len, (s.first + s.n) << p.unit);
+    s.k_end = min(keys_of(len, p), (s.first + s.n) << p.unit);
     go_to(unit + s.n, s.units);
     return s;
   };
@@ -328,6 +345,11 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
   struct Tiles {
     int page0, page1;  // no arrays: a lane that picks one of them would send them through memory
     bool ok0, ok1;
+    int live0, live1;  // CHOSEN: tokens among the 16 keys
+    __device__ __forceinline__ int live(bool upper) const {
+      const int a = live0, b = live1;
+      return upper ? b : a;
+    }
     __device__ __forceinline__ int page(bool upper) const {
       const int a = page0, b = page1;
       return upper ? b : a;
@@ -338,19 +360,40 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
     }
   };
   Stretch at;       // the stretch whose rows are read
-  int lane_page;
+  struct PageRef {
+    int page, live;
+  };
+  PageRef lane_page;
   const uint8_t *k_head, *v_head;
   const char *k_state, *v_state;
+  // the page of a sequence that entry i of a pair's list names, and how many tokens it has from `place` on; -1, 0: none
+  auto entry = [&](const Stretch& s, int i, int place) {
+    if constexpr (CHOSEN) {
+      const int u = p.chosen[s.b * p.ch_sb + s.h * p.ch_sh + i];
+      const bool there = (uint32_t)u < (uint32_t)p.max_pages;
+      const int page = p.table[s.b * p.table_sb + (there ? u : 0)], live = there ? s.tokens - (u << p.shift) - place : 0;
+      return PageRef{live > 0 ? page : -1, live};
+    } else {
+      return PageRef{p.table[s.b * p.table_sb + i], 0};
+    }
+  };
   auto pages_of = [&](const Stretch& s, int j) {
-    return p.table[s.b * p.table_sb + min((s.k_begin + 32 * wave + (j + (lane >> 1)) * UNIT + 16 * (lane & 1)) >> p.shift, p.max_pages - 1)];
+    const int key = s.k_begin + 32 * wave + (j + (lane >> 1)) * UNIT + 16 * (lane & 1);
+    PageRef r = entry(s, min(key, p.cap - 1) >> p.shift, key & mask);
+    if (CHOSEN && key >= s.k_end) r.page = -1;
+    return r;
   };
   auto tiles = [&](int j) {
     if (j > 0 && (j & 31) == 0) {
       lane_page = pages_of(at, j);
-      asm volatile("" : "+v"(lane_page));  // waited for here, not in every pass
+      asm volatile("" : "+v"(lane_page.page));  // waited for here, not in every pass
     }
     Tiles t;
-    const int page0 = __builtin_amdgcn_readlane(lane_page, 2 * (j & 31)), page1 = __builtin_amdgcn_readlane(lane_page, 2 * (j & 31) + 1);
+    const int page0 = __builtin_amdgcn_readlane(lane_page.page, 2 * (j & 31)), page1 = __builtin_amdgcn_readlane(lane_page.page, 2 * (j & 31) + 1);
+    if constexpr (CHOSEN) {
+      t.live0 = __builtin_amdgcn_readlane(lane_page.live, 2 * (j & 31));
+      t.live1 = __builtin_amdgcn_readlane(lane_page.live, 2 * (j & 31) + 1);
+    }
     t.ok0 = (uint32_t)page0 < (uint32_t)p.num_pages;
     t.ok1 = (uint32_t)page1 < (uint32_t)p.num_pages;
     t.page0 = t.ok0 ? page0 : 0;
@@ -413,7 +456,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
   typename R::V v;
   u32x4_t qb[KJ];
   Tiles t;
-  auto start = [&](const Stretch& s, int page) {
+  auto start = [&](const Stretch& s, PageRef page) {
     at = s;
     lane_page = page;
     k_head = p.k + (uint64_t)(uint32_t)s.h * p.k_head;
@@ -440,7 +483,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
     const Stretch now = at;
     const bool more = unit < end;
     Stretch next = now;
-    int next_page = 0;
+    PageRef next_page = {0, 0};
     if (more) {
       next = take();
       next_page = pages_of(next, 0);
@@ -497,9 +540,9 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
     // codes: sum of w (zp - c), the unit of the scales, and its inverse
     float corr = 0.0f, unit_v = 0x1p-126f, per_v = 0x1p126f;
 
-    auto whole = [&](int chunk) { return chunk + 32 <= now.k_end && t.ok0 && t.ok1; };
+    auto whole = [&](int chunk) { return (CHOSEN ? t.live0 >= 16 && t.live1 >= 16 : chunk + 32 <= now.k_end) && t.ok0 && t.ok1; };
     // key `i` of half gi is one of the sequence's
-    auto live = [&](int chunk, int gi, int i) { return t.ok(gi) && chunk + 16 * gi + i < now.k_end; };
+    auto live = [&](int chunk, int gi, int i) { return t.ok(gi) && (CHOSEN ? i < t.live(gi) : chunk + 16 * gi + i < now.k_end); };
     // logits: head m, keys 4 kg + i of the two halves; in log2 units, of codes by to_logit, which is the head's
     auto logits = [&](int chunk, float (&s)[8]) {
       f32x4_t x[2];
@@ -670,7 +713,7 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
       f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma clang loop unroll(disable)
       for (int key = now.k_begin; key < now.k_end; ++key) {
-        const int page = p.table[now.b * p.table_sb + (key >> p.shift)];
+        const int page = entry(now, key >> p.shift, key & mask).page;
         if ((uint32_t)page >= (uint32_t)p.num_pages) continue;
         const uint8_t* row = p.v + (uint64_t)(uint32_t)now.h * p.v_head + (uint64_t)(uint32_t)page * p.v_page + (uint32_t)(key & mask) * p.v_row;
         const u32x2_t pairs = *(const u32x2_t*)(row + 2 * d);
@@ -781,11 +824,11 @@ __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedParams p) {
   if (p.lse && d == 0) p.lse[(int64_t)pair * p.Gr + g] = sum == 0.0f ? -INFINITY : all + fast_log2(sum);
 }
 
-PagedParams params_of(const kvx_paged_decode_args& a) {
+ChosenParams params_of(const kvx_paged_decode_args& a, const kvx_chosen_pages* c) {
   const kvx_pages& g = a.pages;
   const bool plain = kv_is_plain(g.kv_dtype);
   const int es = plain ? 2 : 1;
-  PagedParams p{};
+  ChosenParams p{};
   p.lens = a.lens;
   p.table = a.block_table;
   p.table_sb = a.bt_stride_b;
@@ -793,7 +836,13 @@ PagedParams params_of(const kvx_paged_decode_args& a) {
   p.Hkv = g.Hkv;
   p.shift = __builtin_ctz(g.page_size);
   p.max_pages = a.max_pages;
-  p.cap = a.max_pages << p.shift;
+  p.cap = p.table_cap = a.max_pages << p.shift;
+  if (c) {
+    p.cap = min(c->count, a.max_pages) << p.shift;
+    p.chosen = c->pages;
+    p.ch_sb = c->stride_b;
+    p.ch_sh = c->stride_h;
+  }
   p.num_pages = g.num_pages;
   p.Gr = a.Hq / g.Hkv;
   p.q = (const uint16_t*)a.q;
@@ -839,9 +888,14 @@ PagedParams params_of(const kvx_paged_decode_args& a) {
 bool splits(const PagedParams& p) { return p.cap > (1 << p.unit); }
 
 template <int D>
-void launch_head(const PagedParams& p, int kv_dtype, hipStream_t st) {
+void launch_head(const ChosenParams& p, int kv_dtype, hipStream_t st) {
+  const PagedParams& all = p;
   switch (kv_dtype) {
-#define KVX_PAGES_CASE(KV) case KV: hipLaunchKernelGGL((paged_decode_kernel<D, KV>), dim3(p.workgroups), dim3(NT), 0, st, p); break;
+#define KVX_PAGES_CASE(KV)                                                                                         \
+  case KV:                                                                                                         \
+    if (p.chosen) hipLaunchKernelGGL((paged_decode_kernel<D, KV, true>), dim3(p.workgroups), dim3(NT), 0, st, p);  \
+    else hipLaunchKernelGGL((paged_decode_kernel<D, KV, false>), dim3(p.workgroups), dim3(NT), 0, st, all);        \
+    break;
     KVX_PAGES_CASE(KVX_KV_BF16)
     KVX_PAGES_CASE(KVX_KV_F16)
     KVX_PAGES_CASE(KVX_KV_U8)
@@ -855,8 +909,8 @@ void launch_head(const PagedParams& p, int kv_dtype, hipStream_t st) {
   auto join = [&](auto lanes) {
     constexpr int LANES = decltype(lanes)::value;
     const dim3 grid(rows, (p.Gr * D + 4 * LANES - 1) / (4 * LANES));
-    if (kv_elem_f16(kv_dtype)) hipLaunchKernelGGL((paged_join_kernel<D, true, LANES>), grid, dim3(NT), 0, st, p);
-    else hipLaunchKernelGGL((paged_join_kernel<D, false, LANES>), grid, dim3(NT), 0, st, p);
+    if (kv_elem_f16(kv_dtype)) hipLaunchKernelGGL((paged_join_kernel<D, true, LANES>), grid, dim3(NT), 0, st, all);
+    else hipLaunchKernelGGL((paged_join_kernel<D, false, LANES>), grid, dim3(NT), 0, st, all);
   };
   if (rows <= 64) join(std::integral_constant<int, 16>{});
   else join(std::integral_constant<int, 64>{});
@@ -866,13 +920,13 @@ size_t part_floats(const PagedParams& p, int D) { return (size_t)2 * p.workgroup
 
 }  // namespace
 
-size_t paged_decode_workspace(const kvx_paged_decode_args& a) {
-  const PagedParams p = params_of(a);
+size_t paged_decode_workspace(const kvx_paged_decode_args& a, const kvx_chosen_pages* chosen) {
+  const ChosenParams p = params_of(a, chosen);
   return splits(p) ? 4 * (part_floats(p, a.pages.D) + (size_t)4 * p.workgroups * p.Gr + 2 * p.workgroups) : 0;
 }
 
-int launch_paged_decode(const kvx_paged_decode_args& a, hipStream_t st) {
-  PagedParams p = params_of(a);
+int launch_paged_decode(const kvx_paged_decode_args& a, const kvx_chosen_pages* chosen, hipStream_t st) {
+  ChosenParams p = params_of(a, chosen);
   if (splits(p)) {
     p.part_o = (float*)a.workspace;
     p.part_ml = p.part_o + part_floats(p, a.pages.D);

@@ -1,30 +1,12 @@
 // Rotary position encoding of a ragged batch for gfx950 (HBM-bound, one pass, in place): every token has a position of its own, the pairs of a head are
 // its halves' or interleaved, and may cover its first part alone; the head is normalised first where weights are given.
 //   y = x / (|x|_2 / sqrt(D) + eps) * w;   (a, b) -> (a cos - b sin, b cos + a sin),   in fp32, rounded once.
-#include <type_traits>
-
-#include "kvx_common.h"
+#include "rotary_heads.h"
 
 namespace kvx {
 namespace {
 
 constexpr int NT = 256;
-
-template <int LPR>
-__device__ __forceinline__ float sum_over_row(float v) {
-  auto add = [](float x, auto ctrl) {
-    return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
-  };
-  v = add(v, std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
-  v = add(v, std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
-  v = add(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
-  if constexpr (LPR >= 16) v = add(v, std::integral_constant<int, 0x140>{});  // row_mirror
-  if constexpr (LPR == 32) {
-    const u32pair_t r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);  // the other row of the pair
-    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  }
-  return v;
-}
 
 // A workgroup a token, or several (grid y); LPR = D / 8 lanes a head, which hold 8 values each: pairs never leave a lane. Interleaved pairs lie side by side, and a lane
 // holds a stretch of 8; pairs of halves: four values of either half of the rotated part. Lanes behind that part hold stretches. `rows` heads of a workgroup at a
@@ -66,35 +48,12 @@ __global__ __launch_bounds__(512) void rotary_kernel(const kvx_rotary_args a, co
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int head = begin + i * rows + mine;
-      float y[8] = {elem_lo<F16>(x0[i][0]), elem_hi<F16>(x0[i][0]), elem_lo<F16>(x0[i][1]), elem_hi<F16>(x0[i][1]),
-                    elem_lo<F16>(x1[i][0]), elem_hi<F16>(x1[i][0]), elem_lo<F16>(x1[i][1]), elem_hi<F16>(x1[i][1])};
-      if (a.q_weight) {  // uniform
-        float ss = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
-        const float n = sqrtf(sum_over_row<LPR>(ss)) * factor + a.eps;
-        const float* w = head < a.Hq ? a.q_weight : a.k_weight;
-        const f32x4_t w0 = *(const f32x4_t*)(w + lo), w1 = *(const f32x4_t*)(w + hi);
-        const float inv = 1.0f / n;
-        if (__all(n > 0x1p-120f)) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * (e < 4 ? w0[e] : w1[e - 4]);
-        } else {  // whose inverse is infinite, or NaN
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = y[e] / n * (e < 4 ? w0[e] : w1[e - 4]);
-        }
-      }
-      float z[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = INTERLEAVED ? 2 * e : e, k = INTERLEAVED ? 2 * e + 1 : e + 4;
-        z[j] = turns ? y[j] * cv[e] - y[k] * sv[e] : y[j];
-        z[k] = turns ? y[k] * cv[e] + y[j] * sv[e] : y[k];
-      }
+      u32x2_t z0, z1;
+      turn<D, F16, INTERLEAVED>(x0[i], x1[i], a.q_weight != nullptr, head < a.Hq ? a.q_weight : a.k_weight, lo, hi, turns, cv, sv, factor, a.eps, z0, z1);
       if (head < heads) {
         uint16_t* p = token + head * D;
-        put(u32x2_t{pack_pair<F16>(z[0], z[1]), pack_pair<F16>(z[2], z[3])}, (u32x2_t*)(p + lo));
-        put(u32x2_t{pack_pair<F16>(z[4], z[5]), pack_pair<F16>(z[6], z[7])}, (u32x2_t*)(p + hi));
+        put(z0, (u32x2_t*)(p + lo));
+        put(z1, (u32x2_t*)(p + hi));
       }
     }
     begin += stride;

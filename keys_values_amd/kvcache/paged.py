@@ -16,6 +16,11 @@ position for its whole batch, and the zero rows that ``paged_read`` puts behind 
 stay on the device and are read by the kernels alone, so the calls can be captured into a graph and replayed with others in
 their place (graphs that share a memory pool in the order of their capture, as torch asks for: a later one's tensors may lie where
 an earlier one had its workspace). There is no CPU path.
+
+Long sequences need not be read whole for a token. With the lowest and the highest of each page's keys at hand (``paged_bounds``, twice a row's bytes a page),
+``attention.ops.paged_select`` finds the pages that can matter to a query, and ``attention.ops.paged_decode_chosen`` attends to those. A layer's step is
+then ``paged_append`` (rotation and write in one launch), ``paged_bounds`` of the page written to (``tokens=1``), ``paged_select``, ``paged_decode_chosen``; a pool made
+with ``bounds=True`` has them as methods.
 """
 from typing import Optional, Tuple
 
@@ -48,11 +53,31 @@ def paged_read(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table: 
     return _lib.host().paged_read(key_pages, value_pages, block_table, lens, length, head_size, dtype, quant)
 
 
+def paged_append(qkv: torch.Tensor, n_head: int, n_query_groups: int, head_size: int, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float,
+                 cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, slots: torch.Tensor,
+                 quant: Optional[ops.QuantState] = None, interleaved: bool = False) -> None:
+    """What a layer does with the projections of new tokens, in one launch: ``longctx.ops.rotary_`` of qkv's query heads, in place, and of its key heads on their
+    way to the slots ``slots`` (int64, one a token), to which its value heads go too, as :func:`paged_write` stores them. Bit for bit what the two calls give, but
+    that the key heads of qkv (and its value heads) stay as they are. Tokens of a negative position, or of one behind the tables, are padding: nothing of them is changed or
+    stored, whatever their slot. Those with a position and without a slot have their queries turned."""
+    _lib.host().paged_append(qkv, n_head, n_query_groups, head_size, q_weight, k_weight, eps, cos, sin, positions, key_pages, value_pages, slots, quant, interleaved)
+
+
+def paged_bounds(key_pages: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, tokens: Optional[int] = None,
+                 quant: Optional[ops.QuantState] = None) -> None:
+    """Bring ``bounds`` (num_pages, n_query_groups, 2, head_size), of the rows' type, in line with the pages that hold the last ``tokens`` of the first
+    ``lens`` tokens of every sequence (None: all of them): the lowest [.., 0, :] and the highest [.., 1, :] of the page's keys among these, value by value, of codes as
+    :func:`paged_read` gives their rows. A NaN among the keys makes a bound NaN. ``tokens`` is the most that any sequence has got since the last call: pages of
+    sequences that got fewer are looked at again, which changes nothing. Sequences that share a page should share it whole, or have as many tokens in it."""
+    _lib.host().paged_bounds(key_pages, bounds, block_table, lens, tokens, quant)
+
+
 class PagedKVCacheBuffers:
-    """The pool of one layer and its operators. ``num_bits``: None for plain rows, 8 or 4 for codes. A new pool holds zeros."""
+    """The pool of one layer and its operators. ``num_bits``: None for plain rows, 8 or 4 for codes; ``bounds``: whether it keeps the bounds of its pages' keys, which
+    :meth:`select` goes by. A new pool holds zeros."""
 
     def __init__(self, num_pages: int, page_size: int, n_query_groups: int, head_size: int, dtype: torch.dtype = torch.bfloat16, num_bits: Optional[int] = None,
-                 device: Optional[torch.device] = None):
+                 device: Optional[torch.device] = None, bounds: bool = False):
         if num_pages < 1 or n_query_groups < 1:
             raise ValueError(f"num_pages = {num_pages}, n_query_groups = {n_query_groups}: must be positive")
         if page_size not in PAGE_SIZES:
@@ -75,6 +100,8 @@ class PagedKVCacheBuffers:
         if num_bits is not None:
             self.quant = ops.QuantState(*(torch.zeros(rows, dtype=t, device=self.device) for t in (torch.float32, torch.int32) * 2))
 
+        self.bounds = torch.zeros(num_pages, n_query_groups, 2, head_size, dtype=dtype, device=self.device) if bounds else None
+
     def slots(self, block_table: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """Slots of the tokens at ``positions`` (sequences, tokens) of the sequences of ``block_table``, flat int64; -1 for a negative position and
         for one behind the table. Once per step: the layers share them."""
@@ -92,16 +119,37 @@ class PagedKVCacheBuffers:
         """See :func:`paged_write`."""
         paged_write(key, value, self.k, self.v, slots, self.quant)
 
+    def append(self, qkv: torch.Tensor, n_head: int, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float, cos: torch.Tensor, sin: torch.Tensor,
+               positions: torch.Tensor, slots: torch.Tensor, interleaved: bool = False) -> None:
+        """See :func:`paged_append`."""
+        paged_append(qkv, n_head, self.n_query_groups, self.head_size, q_weight, k_weight, eps, cos, sin, positions, self.k, self.v, slots, self.quant, interleaved)
+
+    def _bounds(self) -> torch.Tensor:
+        if self.bounds is None:
+            raise ValueError("the pool keeps no bounds: make it with bounds=True")
+        return self.bounds
+
+    def update_bounds(self, block_table: torch.Tensor, lens: torch.Tensor, tokens: Optional[int] = None) -> None:
+        """See :func:`paged_bounds`."""
+        paged_bounds(self.k, self._bounds(), block_table, lens, tokens, self.quant)
+
+    def select(self, query: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, count: int, first: int = 1, last: int = 1) -> torch.Tensor:
+        """See :func:`keys_values_amd.attention.ops.paged_select`."""
+        return ops.paged_select(query, self._bounds(), block_table, lens, self.page_size, count, first, last)
+
     def read(self, block_table: torch.Tensor, lens: torch.Tensor, length: int) -> Tuple[torch.Tensor, torch.Tensor]:
         """See :func:`paged_read`."""
         return paged_read(self.k, self.v, block_table, lens, length, self.head_size, self.dtype, self.quant)
 
-    def decode(self, query: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, scale: Optional[float] = None,
-               return_lse: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-        """See :func:`keys_values_amd.attention.ops.paged_decode`."""
-        return ops.paged_decode(query, self.k, self.v, block_table, lens, ops.default_scale(self.head_size) if scale is None else scale, return_lse, self.quant)
+    def decode(self, query: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, scale: Optional[float] = None, return_lse: bool = False,
+               chosen: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+        """See :func:`keys_values_amd.attention.ops.paged_decode`; with ``chosen`` pages :func:`keys_values_amd.attention.ops.paged_decode_chosen`."""
+        scale = ops.default_scale(self.head_size) if scale is None else scale
+        if chosen is not None:
+            return ops.paged_decode_chosen(query, self.k, self.v, block_table, lens, chosen, scale, return_lse, self.quant)
+        return ops.paged_decode(query, self.k, self.v, block_table, lens, scale, return_lse, self.quant)
 
     def size_estimate(self) -> int:
         """Bits that the pool takes."""
-        state = self.quant or ()
-        return sum(8 * t.numel() * t.element_size() for t in (self.k, self.v, *state))
+        more = (*(self.quant or ()), *(() if self.bounds is None else (self.bounds,)))
+        return sum(8 * t.numel() * t.element_size() for t in (self.k, self.v, *more))
