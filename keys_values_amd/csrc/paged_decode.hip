@@ -33,6 +33,7 @@
 #include <type_traits>
 
 #include "key_blocks.h"
+#include "work_shares.h"
 
 namespace kvx {
 namespace {
@@ -81,27 +82,6 @@ __device__ __forceinline__ int keys_of(int len, const Params& p) {
 // Units of a pair of a sequence of `len` tokens: those with keys, and, behind them, as many without as the change to the pair takes the time of.
 template <typename Params>
 __device__ __forceinline__ int units_of(int len, const Params& p, int extra) { return max(1, (keys_of(len, p) + (1 << p.unit) - 1) >> p.unit) + extra; }
-
-// Inclusive sum over the lanes of a wavefront, on the vector ALU.
-__device__ __forceinline__ int scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);  // row_shr:2
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);  // row_shr:4
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);  // row_shr:8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 to the odd rows
-  return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 to the upper half
-}
-
-// The shares of `total` units: workgroup w begins with unit first(w).
-struct Shares {
-  int workgroups, each, rest;
-  __device__ __forceinline__ Shares(int total, int n) : workgroups(n), each(total / n), rest(total - each * n) {}
-  __device__ __forceinline__ int first(int w) const { return min(w, workgroups) * each + min(w, rest); }
-  __device__ __forceinline__ int owner(int unit) const {
-    const int big = rest * (each + 1);
-    return unit < big ? unit / (each + 1) : rest + (unit - big) / each;
-  }
-};
 
 template <int D, int KV>
 struct Rows {

@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "page_rows.h"
+#include "work_shares.h"
 
 namespace kvx {
 namespace {
@@ -107,51 +108,295 @@ __device__ __forceinline__ uint32_t key_of(double sum) {
 struct SelectParams {
   kvx_paged_select_args a;
   uint32_t* keys;  // (B, Hkv, max_pages)
-  int parts;       // workgroups of a (sequence, KV head)
 };
 __device__ __forceinline__ int pages_of_sequence(const kvx_paged_select_args& a, int b) {
   const int len = max(a.lens[b], 0);
   return (int)min(((int64_t)len + a.page_size - 1) / a.page_size, (int64_t)a.max_pages);
 }
 
-constexpr int SCORED = 64;  // pages of a workgroup
-
-// D / 8 lanes a page. Products of 16-bit values are exact in 32 bits, and their sums, in 64, differ with the order by less than what the rounding to 32 sees.
-template <int D, bool F16>
-__global__ __launch_bounds__(NTHREADS) void select_score_kernel(const SelectParams p) {
-  constexpr int LPR = D / 8, ROWS = NTHREADS / LPR;
+// v_mfma_f64_4x4x4, four blocks of 4 pages, 4 heads and 4 values: lane l has a value of page l % 16 (A), of head l % 4 (B), and gets the sum of page
+// 4 (l / 4 % 4) + l / 16 and head l % 4. Products of 16-bit values are exact in 32 bits, and their sums, in 64, differ with the order by less than what the rounding to 32 sees.
+// A wavefront takes 16 pages at a time and has the next 16 on their way meanwhile. Queries wait in LDS as pairs q+, q- of 64 bits, the 16 pairs of an instruction
+// side by side. An instruction takes 16 cycles (v_mfma_f64_16x16x4, four times as much work, a hundred).
+//
+// The pages of all (sequence, KV head) pairs are cut into units and dealt out to a fixed number of workgroups, each a stretch of neighbouring units, as paged_decode does with
+// keys. A grid of all units that the table has room for, whatever the lengths: 93 us for 48 sequences of 300 to 131072 tokens in pages of 16, 28 / 4 heads of 128, 42 as it is.
+// Bounds of 134 MB (8 sequences of 131072 tokens in pages of 32, 32 / 8 heads of 128) take 31 us, 5 of them before the first ones arrive; with two workgroups a compute
+// unit that hold twice as many each 33, with loads past the caches 3 more.
+constexpr int UNIT = NTHREADS / 64 * 16;  // pages
+constexpr int score_workgroups(int D) { return D == 256 ? 2 : 4; }  // a compute unit: what registers leave room for
+template <int D, bool F16, int HEADS /* of the group, in fours */>
+__global__ __launch_bounds__(NTHREADS, score_workgroups(D)) void select_score_kernel(const SelectParams p) {
+  typedef double f64x2_t __attribute__((ext_vector_type(2)));
   const kvx_paged_select_args& a = p.a;
-  const int pair = blockIdx.x / p.parts, part = blockIdx.x - pair * p.parts, b = pair / a.Hkv, h = pair - b * a.Hkv, n = pages_of_sequence(a, b), G = a.Hq / a.Hkv;
-  const int col = threadIdx.x % LPR;
-  for (int i = part * SCORED + threadIdx.x / LPR; i < min((part + 1) * SCORED, n); i += ROWS) {
-    const int page = a.block_table[b * a.bt_stride_b + i];
-    uint32_t key = kNever;
-    if ((uint32_t)page < (uint32_t)a.num_pages) {
-      const uint16_t* at = (const uint16_t*)a.bounds + (int64_t)page * a.b_stride_page + h * a.b_stride_h + 8 * col;
-      const u32x4_t lo = *(const u32x4_t*)at, hi = *(const u32x4_t*)(at + a.b_stride_side);
-      for (int g = 0; g < G; ++g) {
-        const u32x4_t q = *(const u32x4_t*)((const uint16_t*)a.q + b * a.q_stride_b + (int64_t)(h * G + g) * a.q_stride_h + 8 * col);
-        double sum = 0.0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = e & 1 ? elem_hi<F16>(q[e >> 1]) : elem_lo<F16>(q[e >> 1]);
-          const float l = e & 1 ? elem_hi<F16>(lo[e >> 1]) : elem_lo<F16>(lo[e >> 1]), u = e & 1 ? elem_hi<F16>(hi[e >> 1]) : elem_lo<F16>(hi[e >> 1]);
-          sum += (double)(x > 0.0f ? x : 0.0f) * (double)u + (double)(x > 0.0f ? 0.0f : x) * (double)l;
-        }
-#pragma unroll
-        for (int step = 1; step < LPR; step *= 2) sum += __shfl_xor(sum, step, 64);
-        key = max(key, key_of(sum));
-      }
-      if (i < a.first || i >= n - a.last) key = kAlways;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = lane >> 4, B = a.B, Hkv = a.Hkv, G = a.Hq / Hkv;
+  __shared__ __align__(16) f64x2_t qs[HEADS][D / 32][8][4][4];  // value 32 x + 8 kg + j of head 4 f + g at [f][x][j][kg][g]
+
+  // ---- this workgroup's units: every wavefront finds them for itself, 64 sequences at a time
+  const int windows = (B + 63) / 64;
+  auto window = [&](int i) { return 64 * i + lane < B ? pages_of_sequence(a, 64 * i + lane) : 0; };
+  auto units_in = [&](int pages) { return (pages + UNIT - 1) / UNIT; };
+  int lane_pages = 0, mine = 0;  // lane_pages: of sequence (b & ~63) + lane
+  for (int i = 0; i < windows; ++i) {
+    lane_pages = window(i);
+    mine += units_in(lane_pages);
+  }
+  const Shares shares(__builtin_amdgcn_readlane(scan(mine), 63) * Hkv, gridDim.x);
+  int unit = shares.first(blockIdx.x);
+  const int end = shares.first(blockIdx.x + 1);
+  if (unit >= end) return;
+  int b = 0, begin_b = 0;  // the unit's sequence, and the sequence's first unit
+  for (int i = 0, before = 0;; ++i) {
+    if (windows > 1) lane_pages = window(i);
+    mine = units_in(lane_pages);
+    const int upto = before + scan(mine);
+    const unsigned long long behind = __ballot(upto * Hkv > unit);
+    if (behind) {
+      const int at = __builtin_ctzll(behind);
+      b = 64 * i + at;
+      begin_b = __builtin_amdgcn_readlane(upto - mine, at) * Hkv;
+      break;
     }
-    if (col == 0) p.keys[(int64_t)pair * a.max_pages + i] = key;
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+
+  struct Tile {
+    u32x4_t lo[D / 32], hi[D / 32];
+    int page;  // of the pool, of page lane % 16 of the tile; -1: none
+  };
+  for (bool again = false;; again = true) {
+    const int n = __builtin_amdgcn_readlane(lane_pages, b & 63), units = units_in(n);
+    if (units > 0) {
+      const int h = (unit - begin_b) / units, from = unit - begin_b - h * units, count = min(units - from, end - unit), pair = b * Hkv + h;
+      const int last = min(n, (from + count) * UNIT);
+      const int* table = a.block_table + b * a.bt_stride_b;
+      const uint16_t* bounds = (const uint16_t*)a.bounds + h * a.b_stride_h + 8 * kg;
+      auto entry = [&](int first) { return table[min(first + (lane & 15), n - 1)]; };
+      auto load = [&](Tile& r, int entry, int first) {
+        r.page = first + (lane & 15) < last && (uint32_t)entry < (uint32_t)a.num_pages ? entry : -1;
+        const uint16_t* at = bounds + (int64_t)max(r.page, 0) * a.b_stride_page;
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {
+          r.lo[x] = *(const u32x4_t*)(at + 32 * x);
+          r.hi[x] = *(const u32x4_t*)(at + a.b_stride_side + 32 * x);
+        }
+      };
+      auto score = [&](const Tile& r, int first) {
+        asm volatile("" ::: "memory");  // the queries are read anew, not held in registers, of which there are too few
+        double up[HEADS], down[HEADS];
+#pragma unroll
+        for (int f = 0; f < HEADS; ++f) up[f] = down[f] = 0.0;
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const double l = j & 1 ? elem_hi<F16>(r.lo[x][j >> 1]) : elem_lo<F16>(r.lo[x][j >> 1]), u = j & 1 ? elem_hi<F16>(r.hi[x][j >> 1]) : elem_lo<F16>(r.hi[x][j >> 1]);
+#pragma unroll
+            for (int f = 0; f < HEADS; ++f) {
+              const f64x2_t q = qs[f][x][j][kg][lane & 3];
+              up[f] = __builtin_amdgcn_mfma_f64_4x4x4f64(u, q[0], up[f], 0, 0, 0);
+              down[f] = __builtin_amdgcn_mfma_f64_4x4x4f64(l, q[1], down[f], 0, 0, 0);
+            }
+          }
+        uint32_t key = kNever;
+#pragma unroll
+        for (int f = 0; f < HEADS; ++f)
+          if (4 * f + (lane & 3) < G) key = max(key, key_of(up[f] + down[f]));
+        key = max(key, (uint32_t)__builtin_amdgcn_mov_dpp((int)key, 0xB1, 0xf, 0xf, true));  // quad_perm [1,0,3,2]
+        key = max(key, (uint32_t)__builtin_amdgcn_mov_dpp((int)key, 0x4E, 0xf, 0xf, true));  // quad_perm [2,3,0,1]
+        const int mine = (lane & 12) + kg, i = first + mine;  // the page whose sums this lane has
+        const unsigned long long pages = __ballot(r.page >= 0);
+        if (!((pages >> mine) & 1)) key = kNever;
+        else if (i < a.first || i >= n - a.last) key = kAlways;
+        if ((lane & 3) == 0 && i < last) p.keys[(int64_t)pair * a.max_pages + i] = key;
+      };
+      // A tile's entries of the table are read one tile ahead of its bounds, and before those of the tile in between: what waits for them waits for nothing else. Behind the
+      // last page, page 0 of the pool is read: loads under a condition would have to be waited for whether they are there or not.
+      int first = from * UNIT + wave * 16;
+      int next = entry(first), then = entry(first + UNIT);
+      Tile one, two;
+      if (again) __syncthreads();  // the queries before are read
+      for (int i = threadIdx.x; i < 4 * HEADS * (D / 8); i += NTHREADS) {
+        const int g = i % (4 * HEADS), col = i / (4 * HEADS);
+        u32x4_t q = {0u, 0u, 0u, 0u};
+        if (g < G) q = *(const u32x4_t*)((const uint16_t*)a.q + b * a.q_stride_b + (int64_t)(h * G + g) * a.q_stride_h + 8 * col);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float x = j & 1 ? elem_hi<F16>(q[j >> 1]) : elem_lo<F16>(q[j >> 1]);
+          qs[g >> 2][col >> 2][j][col & 3][g & 3] = f64x2_t{x > 0.0f ? x : 0.0f, x > 0.0f ? 0.0f : x};  // a NaN is the second's
+        }
+      }
+      load(one, next, first);
+      __syncthreads();
+      for (; first < last; first += 2 * UNIT) {
+        next = entry(first + 2 * UNIT);
+        __builtin_amdgcn_sched_barrier(0);
+        load(two, then, first + UNIT);
+        __builtin_amdgcn_sched_barrier(0);
+        score(one, first);
+        if (first + UNIT >= last) break;
+        __builtin_amdgcn_sched_barrier(0);
+        then = entry(first + 3 * UNIT);
+        __builtin_amdgcn_sched_barrier(0);
+        load(one, next, first + 2 * UNIT);
+        __builtin_amdgcn_sched_barrier(0);
+        score(two, first + UNIT);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      unit += count;
+      if (unit >= end) break;
+    }
+    if (unit == begin_b + units * Hkv) {
+      begin_b = unit;
+      ++b;
+      if ((b & 63) == 0 && b < B) lane_pages = window(b >> 6);
+    }
   }
 }
 
-// The `count` largest keys of a (sequence, KV head), of equal ones the first, in order of their pages: the last key that is taken is found from its upper bits
-// down, by counting.
+// The `count` largest keys of a (sequence, KV head), of equal ones the first, in order of their pages, for up to R * NT pages, whose keys stay in registers. The last key that is taken lies
+// in one of 2048 equal parts of the keys' range, found by counting, then in one of 2048 parts of that, until no more of its part are left over (after three times a part is
+// one key). By their upper bits instead, as the long form does, most keys would count in the same few places, one after the other.
+template <int R, int NT>
+__global__ __launch_bounds__(NT) void select_choose_kernel(const SelectParams p) {
+  constexpr int BINS = 2048, WAVES = NT / 64, EACH = BINS / NT;  // EACH: parts a lane counts up, from the largest down
+  const kvx_paged_select_args& a = p.a;
+  const int pair = blockIdx.x, b = pair / a.Hkv, n = pages_of_sequence(a, b), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ int counts[BINS], sums[WAVES], at_bin, at_rest, at_count;
+  __shared__ uint32_t lows[WAVES], highs[WAVES];
+  __shared__ int places[R * WAVES];
+  const uint32_t* keys = p.keys + (int64_t)pair * a.max_pages;
+  int32_t* out = a.chosen + (int64_t)pair * a.count;
+  uint32_t key[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) key[r] = r * NT + tid < n ? keys[r * NT + tid] : kNever;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) counts[NT * e + tid] = 0;
+  // ---- range of the keys that are neither taken anyway nor left out, and the numbers of those (in both halves of a word of their own: n < 2^26)
+  uint32_t low = kAlways, high = kNever;
+  int always = 0, others = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const bool other = key[r] != kNever && key[r] != kAlways;
+    if (other) {
+      low = min(low, key[r]);
+      high = max(high, key[r]);
+    }
+    always += __popcll(__ballot(key[r] == kAlways));
+    others += __popcll(__ballot(other));
+  }
+#pragma unroll
+  for (int step = 1; step < 64; step *= 2) {
+    low = min(low, (uint32_t)__shfl_xor((int)low, step, 64));
+    high = max(high, (uint32_t)__shfl_xor((int)high, step, 64));
+  }
+  if (lane == 0) {
+    lows[wave] = low;
+    highs[wave] = high;
+    sums[wave] = always << 16 | others;  // at most R * 64 each, which is 2048
+  }
+  __syncthreads();
+  always = others = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    low = min(low, lows[w]);
+    high = max(high, highs[w]);
+    always += sums[w] >> 16;
+    others += sums[w] & 0xffff;
+  }
+  // ---- `from`: the least key that is taken; `rest` of the keys equal to it, where there are more
+  int rest = a.count - always;
+  uint32_t from = low;
+  bool part = false;  // not all of the last keys are taken
+  if (rest <= 0) {
+    from = kAlways;
+  } else if (others > rest) {
+    const int width = 32 - __builtin_clz((high - low) | 1u);
+    int shift = max(0, width - 11);
+    uint32_t to = high;  // the keys that are looked at: from .. to
+    for (;;) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (key[r] >= from && key[r] <= to) atomicAdd(&counts[(key[r] - from) >> shift], 1);
+      __syncthreads();
+      int c[EACH], all = 0;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        c[e] = counts[BINS - 1 - EACH * tid - e];
+        all += c[e];
+      }
+      int upto = scan(all);
+      if (lane == 63) sums[wave] = upto;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) upto += w < wave ? sums[w] : 0;
+      if (upto - all < rest && rest <= upto) {
+        int before = upto - all;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          if (before < rest && rest <= before + c[e]) {
+            at_bin = BINS - 1 - EACH * tid - e;
+            at_rest = rest - before;
+            at_count = c[e];
+          }
+          before += c[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) counts[BINS - 1 - EACH * tid - e] = 0;
+      __syncthreads();
+      rest = at_rest;
+      from += (uint32_t)at_bin << shift;
+      to = from + min((1u << shift) - 1, high - from);
+      part = at_count > rest;
+      if (!part || shift == 0) break;
+      shift = max(0, shift - 11);
+    }
+  }
+  // ---- what is taken, in order
+  bool take[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) take[r] = key[r] != kNever && key[r] >= from;
+  auto place = [&](const bool (&of)[R], int (&to)[R]) {  // places among those of all wavefronts and rows; returns how many there are
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const unsigned long long m = __ballot(of[r]);
+      to[r] = __popcll(m & ((1ull << lane) - 1));
+      if (lane == 0) places[r * WAVES + wave] = __popcll(m);
+    }
+    __syncthreads();
+    int before = 0, mine[R];
+    for (int first = 0; first < R * WAVES; first += 64) {
+      const int x = first + lane < R * WAVES ? places[first + lane] : 0, y = scan(x);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (r * WAVES + wave >= first && r * WAVES + wave < first + 64) mine[r] = before + __shfl(y - x, r * WAVES + wave - first, 64);
+      before += __shfl(y, 63, 64);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) to[r] += mine[r];
+    __syncthreads();
+    return before;
+  };
+  int to[R];
+  if (part) {
+    bool tie[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) tie[r] = key[r] == from;
+    place(tie, to);
+#pragma unroll
+    for (int r = 0; r < R; ++r) take[r] = take[r] && (key[r] != from || to[r] < rest);
+  }
+  const int taken = place(take, to);
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (take[r] && to[r] < a.count) out[to[r]] = r * NT + tid;
+  for (int i = taken + tid; i < a.count; i += NT) out[i] = -1;
+}
+
+// The same for any number of pages, whose keys are read again and again: the last key that is taken is found from its upper bits down, by counting.
 constexpr int CHOOSERS = 1024;
-__global__ __launch_bounds__(CHOOSERS) void select_choose_kernel(const SelectParams p) {
+__global__ __launch_bounds__(CHOOSERS) void select_choose_long_kernel(const SelectParams p) {
   const kvx_paged_select_args& a = p.a;
   const int pair = blockIdx.x, b = pair / a.Hkv, n = pages_of_sequence(a, b), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   constexpr int WAVES = CHOOSERS / 64, BINS = 2048;
@@ -252,19 +497,43 @@ int launch_paged_bounds(const kvx_paged_bounds_args& a, hipStream_t st) {
 size_t paged_select_workspace(const kvx_paged_select_args& a) { return (size_t)4 * a.B * a.Hkv * a.max_pages; }
 
 int launch_paged_select(const kvx_paged_select_args& a, hipStream_t st) {
-  const SelectParams p = {a, (uint32_t*)a.workspace, (a.max_pages + SCORED - 1) / SCORED};
-  const int64_t blocks = (int64_t)a.B * a.Hkv * p.parts;
-  KVX_REQUIRE(blocks < (1 << 23) && (int64_t)a.B * a.Hkv < (1 << 21), KVX_ERR_UNSUPPORTED, "kvx_paged_select: %d sequences of up to %d pages, %d KV heads in one call", a.B,
-              a.max_pages, a.Hkv);
-  const dim3 grid((unsigned)blocks);
-  auto go = [&](auto d) {
-    if (a.elem_dtype == KVX_KV_F16) hipLaunchKernelGGL((select_score_kernel<decltype(d)::value, true>), grid, dim3(NTHREADS), 0, st, p);
-    else hipLaunchKernelGGL((select_score_kernel<decltype(d)::value, false>), grid, dim3(NTHREADS), 0, st, p);
+  const SelectParams p = {a, (uint32_t*)a.workspace};
+  const int64_t count = (int64_t)a.B * a.Hkv, units = count * ((a.max_pages + UNIT - 1) / UNIT);
+  KVX_REQUIRE(count < (1 << 21) && units < (1 << 30), KVX_ERR_UNSUPPORTED, "kvx_paged_select: %d sequences of up to %d pages, %d KV heads in one call", a.B, a.max_pages,
+              a.Hkv);
+  const unsigned blocks = (unsigned)min(units, (int64_t)score_workgroups(a.D) * num_cus());
+  const int group = a.Hq / a.Hkv;
+  auto go = [&](auto d, auto f16) {
+    auto score = [&](auto heads) {
+      hipLaunchKernelGGL((select_score_kernel<decltype(d)::value, decltype(f16)::value, decltype(heads)::value>), dim3(blocks), dim3(NTHREADS), 0, st, p);
+    };
+    if (group <= 4) score(std::integral_constant<int, 1>{});
+    else if (group <= 8) score(std::integral_constant<int, 2>{});
+    else score(std::integral_constant<int, 4>{});
   };
-  if (a.D == 256) go(std::integral_constant<int, 256>{});
-  else if (a.D == 128) go(std::integral_constant<int, 128>{});
-  else go(std::integral_constant<int, 64>{});
-  hipLaunchKernelGGL(select_choose_kernel, dim3((unsigned)(a.B * a.Hkv)), dim3(CHOOSERS), 0, st, p);
+  auto go_type = [&](auto d) {
+    if (a.elem_dtype == KVX_KV_F16) go(d, std::true_type{});
+    else go(d, std::false_type{});
+  };
+  if (a.D == 256) go_type(std::integral_constant<int, 256>{});
+  else if (a.D == 128) go_type(std::integral_constant<int, 128>{});
+  else go_type(std::integral_constant<int, 64>{});
+  const dim3 pairs((unsigned)(a.B * a.Hkv));
+  // 512 lanes take less time than 1024 up to 2048 pages, as long at 4096, and more beyond: 1024 pages 4.2 and 5.0 us, 4096 5.9 and 5.9, 8192 7.0 and 6.7
+  auto choose = [&](auto r, auto nt) {
+    constexpr int R = decltype(r)::value, NT = decltype(nt)::value;
+    hipLaunchKernelGGL((select_choose_kernel<R, NT>), pairs, dim3(NT), 0, st, p);
+  };
+  const std::integral_constant<int, 512> few;
+  const std::integral_constant<int, 1024> many;
+  if (a.max_pages <= 512) choose(std::integral_constant<int, 1>{}, few);
+  else if (a.max_pages <= 1024) choose(std::integral_constant<int, 2>{}, few);
+  else if (a.max_pages <= 2048) choose(std::integral_constant<int, 4>{}, few);
+  else if (a.max_pages <= 4096) choose(std::integral_constant<int, 4>{}, many);
+  else if (a.max_pages <= 8192) choose(std::integral_constant<int, 8>{}, many);
+  else if (a.max_pages <= 16384) choose(std::integral_constant<int, 16>{}, many);
+  else if (a.max_pages <= 32768) choose(std::integral_constant<int, 32>{}, many);
+  else hipLaunchKernelGGL(select_choose_long_kernel, pairs, dim3(CHOOSERS), 0, st, p);
   KVX_HIP(hipGetLastError());
   return KVX_OK;
 }
