@@ -13,84 +13,199 @@ namespace {
 __device__ __forceinline__ float lowest(float a, float b) { return __builtin_elementwise_minimum(a, b); }
 __device__ __forceinline__ float highest(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// A wavefront a (page, KV head) or, for larger pages, several; D / 8 lanes a row. Block: W wavefronts.
+// min / max over the halves of a wavefront, then over the rows of 16 of a half, of two registers at a time: lanes trade the half (or row) of one register for that of the
+// other, so that a result has both. x[] shrinks by half with every step.
+template <int N, typename F>
+__device__ __forceinline__ void fold_halves(float (&x)[N], F best) {
+#pragma unroll
+  for (int e = 0; e < N / 2; ++e) {
+    const u32pair_t r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[e]), __float_as_uint(x[e + N / 2]), false, false);
+    x[e] = best(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+}
+template <int N, typename F>
+__device__ __forceinline__ void fold_rows(float (&x)[N], F best) {  // of x[0 .. N / 2)
+#pragma unroll
+  for (int e = 0; e < N / 4; ++e) {
+    const u32pair_t r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[e]), __float_as_uint(x[e + N / 4]), false, false);
+    x[e] = best(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+}
+
+// W wavefronts a (page, KV head); D / 8 lanes a row, U rows a lane at a time. HBM-bound. The pages of all sequences are dealt out to a fixed number of workgroups, a stretch of
+// neighbouring (page, head) each, and a wavefront has the first rows of its next one on their way while it folds one. A page's last rows are looked at again in place of those that it does
+// not have: all loads of a step are on their way before the first is waited for.
+// 142000 tokens in pages of 16, 8 heads of 128 (290 MB of keys, 37 of bounds): 64 us, with loads through the caches 71. A grid of all pages that the tables have room for takes 63
+// there, but longer the emptier the tables are.
 template <int D, int KV, int W>
-__global__ __launch_bounds__(64 * W) void paged_bounds_kernel(const kvx_paged_bounds_args a, const int shift, const int most) {
+__global__ __launch_bounds__(W == 16 ? 1024 : 256) void paged_bounds_kernel(const kvx_paged_bounds_args a, const int shift) {
   constexpr bool PLAIN = kv_is_plain(KV), U4 = kv_is_u4(KV), F16 = kv_elem_f16(KV);
-  constexpr int LPR = D / 8, ROWS = 64 * W / LPR, ES = PLAIN ? 2 : 1;
+  constexpr int LPR = D / 8, ROWS = 64 / LPR, ES = PLAIN ? 2 : 1, U = 4, NT = W == 16 ? 1024 : 256, AT_ONCE = NT / 64 / W;
   const kvx_pages& p = a.pages;
-  const int64_t item = blockIdx.x;
-  const int h = (int)(item % p.Hkv), j = (int)(item / p.Hkv % most), b = (int)(item / p.Hkv / most);
-  const int cap = a.max_pages << shift, len = min(max(a.lens[b], 0), cap);
-  const int i = ((len + p.page_size - 1) >> shift) - 1 - j;  // the sequence's page, from the last one back
-  if (i < 0 || (int64_t)(i + 1) * p.page_size <= (int64_t)len - a.tokens) return;
-  const int page = a.block_table[b * a.bt_stride_b + i];
-  if ((uint32_t)page >= (uint32_t)p.num_pages) return;
-  const int rows = min(len - (i << shift), p.page_size), col = threadIdx.x % LPR, first = threadIdx.x / LPR;
-  const uint8_t* k = (const uint8_t*)p.k + ((int64_t)page * p.k_stride_page + h * p.k_stride_h) * ES;
-  const int64_t q = (int64_t)page * p.qs_stride_page + h * p.qs_stride_h;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, B = a.B, Hkv = p.Hkv, cap = a.max_pages << shift;
+
+  // ---- this workgroup's share: every wavefront finds it for itself, 64 sequences at a time
+  const int windows = (B + 63) / 64;
+  auto window = [&](int i) { return 64 * i + lane < B ? min(max(a.lens[64 * i + lane], 0), cap) : 0; };
+  auto begin_of = [&](int len) { return max(len - a.tokens, 0) >> shift; };  // the first page that is looked at
+  auto pages_in = [&](int len) { return ((len + p.page_size - 1) >> shift) - begin_of(len); };
+  int lane_len = 0, mine = 0;  // lane_len: of sequence (b & ~63) + lane
+  for (int i = 0; i < windows; ++i) {
+    lane_len = window(i);
+    mine += pages_in(lane_len);
+  }
+  const Shares shares(__builtin_amdgcn_readlane(scan(mine), 63) * Hkv, gridDim.x);
+  int unit = shares.first(blockIdx.x) + wave / W;
+  const int end = shares.first(blockIdx.x + 1);
+  if (unit >= end) return;  // all wavefronts of a (page, head), which are all of the workgroup where they wait for each other
+  int b = 0, begin_b = 0;   // the unit's sequence, and the sequence's first unit
+  for (int i = 0, before = 0;; ++i) {
+    if (windows > 1) lane_len = window(i);
+    mine = pages_in(lane_len);
+    const int upto = before + scan(mine);
+    const unsigned long long behind = __ballot(upto * Hkv > unit);
+    if (behind) {
+      const int at = __builtin_ctzll(behind);
+      b = 64 * i + at;
+      begin_b = __builtin_amdgcn_readlane(upto - mine, at) * Hkv;
+      break;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+
+  const int col = lane % LPR;
+  struct Item {
+    int entry, h, rows;  // of the table; rows that hold tokens
+  };
+  auto item_of = [&](int unit) {  // units come in rising order
+    for (;;) {
+      const int len = __builtin_amdgcn_readlane(lane_len, b & 63), units = pages_in(len) * Hkv;
+      if (unit < begin_b + units) {
+        const int i = (unit - begin_b) / Hkv, page = begin_of(len) + i;
+        return Item{a.block_table[b * a.bt_stride_b + page], unit - begin_b - i * Hkv, min(len - (page << shift), p.page_size)};
+      }
+      begin_b += units;
+      ++b;
+      if ((b & 63) == 0) lane_len = window(b >> 6);
+    }
+  };
+  struct Step {
+    u32x4_t w[U];
+    float scale[U];
+    int32_t zp[U];
+  };
+  auto load = [&](Step& s, const Item& t, int r0) {
+    const int64_t page = (uint32_t)t.entry < (uint32_t)p.num_pages ? t.entry : 0;  // of a page that the pool does not have nothing is kept
+    const uint8_t* k = (const uint8_t*)p.k + (page * p.k_stride_page + t.h * p.k_stride_h) * ES + (PLAIN ? 16 * col : U4 ? (int)u4_byte_off<D>(col) : 8 * col);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = min(r0 + u * ROWS + lane / LPR, t.rows - 1);
+      const uint8_t* at = k + (uint32_t)r * (uint32_t)(p.k_stride_t * ES);
+      if constexpr (PLAIN) {
+        s.w[u] = __builtin_nontemporal_load((const u32x4_t*)at);
+      } else {
+        const u32x2_t c = __builtin_nontemporal_load((const u32x2_t*)at);
+        s.w[u] = u32x4_t{c[0], c[1], 0u, 0u};
+        const int64_t q = page * p.qs_stride_page + t.h * p.qs_stride_h + r;
+        s.scale[u] = p.k_scale[q];
+        s.zp[u] = p.k_zp[q];
+      }
+    }
+  };
   float lo[8], hi[8];
+  auto take = [&](const Step& s) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    lo[e] = INFINITY;
-    hi[e] = -INFINITY;
-  }
-  for (int r = first; r < rows; r += ROWS) {
-    const uint8_t* at = k + (int64_t)r * p.k_stride_t * ES;
-    float x[8];
-    if constexpr (PLAIN) {
-      const u32x4_t w = *(const u32x4_t*)(at + 16 * col);
+    for (int u = 0; u < U; ++u) {
+      float x[8];
+      if constexpr (PLAIN) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[2 * e] = elem_lo<F16>(w[e]);
-        x[2 * e + 1] = elem_hi<F16>(w[e]);
+        for (int e = 0; e < 4; ++e) {
+          x[2 * e] = elem_lo<F16>(s.w[u][e]);
+          x[2 * e + 1] = elem_hi<F16>(s.w[u][e]);
+        }
+      } else {
+        u32x2_t c = {s.w[u][0], s.w[u][1]};
+        if constexpr (U4) c = u4_codes(c, u4_shift<D>(col));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (float)((int32_t)((c[e >> 2] >> (8 * (e & 3))) & 0xff) - s.zp[u]) * s.scale[u];
       }
-    } else {
-      u32x2_t c = *(const u32x2_t*)(at + (U4 ? (int)u4_byte_off<D>(col) : 8 * col));
-      if constexpr (U4) c = u4_codes(c, u4_shift<D>(col));
-      const float scale = p.k_scale[q + r];
-      const int32_t zp = p.k_zp[q + r];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (float)((int32_t)((c[e >> 2] >> (8 * (e & 3))) & 0xff) - zp) * scale;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      lo[e] = lowest(lo[e], x[e]);
-      hi[e] = highest(hi[e], x[e]);
-    }
-  }
-#pragma unroll
-  for (int step = LPR; step < 64; step *= 2) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      lo[e] = lowest(lo[e], __shfl_xor(lo[e], step, 64));
-      hi[e] = highest(hi[e], __shfl_xor(hi[e], step, 64));
-    }
-  }
-  if constexpr (W > 1) {
-    __shared__ float joined[W][2][D];
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) < LPR) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        joined[wave][0][8 * col + e] = lo[e];
-        joined[wave][1][8 * col + e] = hi[e];
+        lo[e] = lowest(lo[e], x[e]);
+        hi[e] = highest(hi[e], x[e]);
       }
     }
-    __syncthreads();
-    if (threadIdx.x >= LPR) return;
-    for (int w = 1; w < W; ++w) {
+  };
+  // over the lanes of a value: a lane keeps VALUES of its 8, from `first` on
+  constexpr int VALUES = D == 256 ? 4 : 2;
+  auto fold = [&](float (&x)[8], auto best) {
+    fold_halves(x, best);
+    if constexpr (D <= 128) fold_rows(x, best);
+    if constexpr (D == 64)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        lo[e] = lowest(lo[e], joined[w][0][8 * col + e]);
-        hi[e] = highest(hi[e], joined[w][1][8 * col + e]);
-      }
+      for (int e = 0; e < VALUES; ++e) x[e] = best(x[e], __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x[e]), 0x128, 0xf, 0xf, true)));  // row_ror:8
+  };
+  const int first = 8 * col + (D == 256 ? lane >> 5 << 2 : lane >> 4 << 1);
+  auto bounds_of = [&](const Item& t, Step& s) {  // s: the first rows
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      lo[e] = INFINITY;
+      hi[e] = -INFINITY;
     }
+    for (int r0 = wave % W * ROWS * U;;) {
+      take(s);
+      r0 += W * ROWS * U;
+      if (r0 >= t.rows) break;
+      load(s, t, r0);
+    }
+    fold(lo, lowest);
+    fold(hi, highest);
+    if constexpr (W > 1) {
+      __shared__ __align__(16) float joined[NT / 64][2][D];
+#pragma unroll
+      for (int e = 0; e < VALUES; ++e) {
+        joined[wave][0][first + e] = lo[e];
+        joined[wave][1][first + e] = hi[e];
+      }
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll 3
+        for (int w = 1; w < W; ++w)
+#pragma unroll
+          for (int e = 0; e < VALUES; ++e) {
+            lo[e] = lowest(lo[e], joined[w][0][first + e]);
+            hi[e] = highest(hi[e], joined[w][1][first + e]);
+          }
+      }
+      __syncthreads();
+      if (wave != 0) return;
+    }
+    if ((uint32_t)t.entry >= (uint32_t)p.num_pages || (D == 64 && (lane & 8))) return;
+    uint16_t* to = (uint16_t*)a.bounds + (int64_t)t.entry * a.b_stride_page + t.h * a.b_stride_h + first;
+#pragma unroll
+    for (int e = 0; e < VALUES; e += 2) {
+      *(uint32_t*)(to + e) = pack_pair<F16>(lo[e], lo[e + 1]);
+      *(uint32_t*)(to + a.b_stride_side + e) = pack_pair<F16>(hi[e], hi[e + 1]);
+    }
+  };
+  Step one, two;
+  Item now = item_of(unit), next = now, then = now;  // behind the last, the last one is read again
+  if (unit + AT_ONCE < end) next = then = item_of(unit + AT_ONCE);
+  load(one, now, wave % W * ROWS * U);
+  for (;; unit += 2 * AT_ONCE) {
+    if (unit + 2 * AT_ONCE < end) then = item_of(unit + 2 * AT_ONCE);
+    load(two, next, wave % W * ROWS * U);
+    __builtin_amdgcn_sched_barrier(0);
+    bounds_of(now, one);
+    if (unit + AT_ONCE >= end) break;
+    now = then;
+    if (unit + 3 * AT_ONCE < end) then = item_of(unit + 3 * AT_ONCE);
+    load(one, now, wave % W * ROWS * U);
+    __builtin_amdgcn_sched_barrier(0);
+    bounds_of(next, two);
+    if (unit + 2 * AT_ONCE >= end) break;
+    next = then;
   }
-  if (threadIdx.x >= LPR) return;
-  uint16_t* to = (uint16_t*)a.bounds + (int64_t)page * a.b_stride_page + h * a.b_stride_h + 8 * col;
-  *(u32x4_t*)to = u32x4_t{pack_pair<F16>(lo[0], lo[1]), pack_pair<F16>(lo[2], lo[3]), pack_pair<F16>(lo[4], lo[5]), pack_pair<F16>(lo[6], lo[7])};
-  *(u32x4_t*)(to + a.b_stride_side) = u32x4_t{pack_pair<F16>(hi[0], hi[1]), pack_pair<F16>(hi[2], hi[3]), pack_pair<F16>(hi[4], hi[5]), pack_pair<F16>(hi[6], hi[7])};
 }
 
 // ---- the choice ------------------------------------------------------------------------------------------------------------------
@@ -483,8 +598,10 @@ int launch_paged_bounds(const kvx_paged_bounds_args& a, hipStream_t st) {
   KVX_REQUIRE(items < (1 << 22), KVX_ERR_UNSUPPORTED, "kvx_paged_bounds: %d sequences of up to %d pages, %d KV heads in one call", a.B, most, p.Hkv);
   by_store(p, [&](auto d, auto kv) {
     auto go = [&](auto w) {
-      hipLaunchKernelGGL((paged_bounds_kernel<decltype(d)::value, decltype(kv)::value, decltype(w)::value>), dim3((unsigned)items), dim3(64 * decltype(w)::value), 0, st, a,
-                         __builtin_ctz(p.page_size), most);
+      constexpr int W = decltype(w)::value, NT = W == 16 ? 1024 : 256;
+      constexpr int64_t each = NT / 64 / W;
+      const int64_t blocks = min((items + each - 1) / each, (int64_t)(W == 16 ? 1 : 5) * num_cus());  // what registers leave room for
+      hipLaunchKernelGGL((paged_bounds_kernel<decltype(d)::value, decltype(kv)::value, W>), dim3((unsigned)blocks), dim3(NT), 0, st, a, __builtin_ctz(p.page_size));
     };
     if (p.page_size <= 32) go(std::integral_constant<int, 1>{});
     else if (p.page_size <= 128) go(std::integral_constant<int, 4>{});

@@ -42,9 +42,9 @@ __device__ __forceinline__ void turn(u32x2_t x0, u32x2_t x1, bool norm, const fl
     if (__all(n > 0x1p-120f)) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * (e < 4 ? w0[e] : w1[e - 4]);
-    } else {  // whose inverse is infinite, or NaN
+    } else {  // some whose inverse is infinite, or NaN
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = y[e] / n * (e < 4 ? w0[e] : w1[e - 4]);
+      for (int e = 0; e < 8; ++e) y[e] = (n > 0x1p-120f ? y[e] * inv : y[e] / n) * (e < 4 ? w0[e] : w1[e - 4]);
     }
   }
   float z[8];
