@@ -851,6 +851,11 @@ ChosenParams params_of(const kvx_paged_decode_args& a, const kvx_chosen_pages* c
   p.lse = a.lse;
   // Tables of up to 512 tokens: a pair is a workgroup's, and there is no second launch.
   p.unit = p.cap <= 4 * UNIT ? 9 : 7;
+  // Lists of pages are mostly full, so that pairs have as much work each: where they are enough to keep the units busy, a list of up to 2048 tokens is a workgroup's too. 64 pages of
+  // 16, 32 / 8 heads of 128, kernel and join or kernel alone: 24 sequences, plain 28.4 and 24.1 us, 32 32.7 and 27.9, 64 56.2 and 51.4, 8-bit 32 26.2 and 20.0; but 8
+  // sequences, plain, 16.6 and 19.8. Where most sequences have few tokens the longest list takes longer than it would in parts (1024 plain keys 20 us, 13 and 4 in parts).
+  const int64_t lists = (int64_t)a.B * g.Hkv;
+  if (c && p.cap > 4 * UNIT && p.cap <= 2048 && 4 * lists >= p.cap) p.unit = 32 - __builtin_clz(p.cap - 1);
   // Beginning a pair of codes takes the time of one unit of 8-bit rows, or two of 4-bit ones: it counts as such, or the workgroups that get the short pairs come last. 92
   // sequences of lengths even in the logarithm from 15 to 9560, 4-bit rows of 128, 32 / 4 heads: 40.8 us without, 29.6 with one unit, 26.2 with two; 14 from 25 to 35609, 8-bit
   // rows of 256: 76.8 without, 63.1 with one or two. Plain rows, whose units take longer, only lose: 200 of 1 to 3000, 65.8 without, 68.5 with one.

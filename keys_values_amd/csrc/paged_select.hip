@@ -210,7 +210,7 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void paged_bounds_kernel(cons
 
 // ---- the choice ------------------------------------------------------------------------------------------------------------------
 
-constexpr uint32_t kNever = 0u, kInfinite = 0xfffffffeu, kAlways = 0xffffffffu;
+constexpr uint32_t kNever = 0u, kInfinite = 0xfffffffdu, kAlways = 0xfffffffeu;
 
 // Keys of scores: unsigned numbers in their order, between kNever and kInfinite. What is not finite counts as infinite.
 __device__ __forceinline__ uint32_t key_of(double sum) {
@@ -239,13 +239,115 @@ __device__ __forceinline__ int pages_of_sequence(const kvx_paged_select_args& a,
 // Bounds of 134 MB (8 sequences of 131072 tokens in pages of 32, 32 / 8 heads of 128) take 31 us, 5 of them before the first ones arrive; with two workgroups a compute
 // unit that hold twice as many each 33, with loads past the caches 3 more.
 constexpr int UNIT = NTHREADS / 64 * 16;  // pages
+
+// What a wavefront scores 16 pages of one (sequence, KV head) with; `q`: the queries in LDS
+template <int D, bool F16, int HEADS /* of the group, in fours */>
+struct Scorer {
+  typedef double f64x2_t __attribute__((ext_vector_type(2)));
+  typedef f64x2_t Queries[HEADS][D / 32][8][4][4];  // value 32 x + 8 kg + j of head 4 f + g at [f][x][j][kg][g]
+  struct Tile {
+    u32x4_t lo[D / 32], hi[D / 32];
+    int page;  // of the pool, of page lane % 16 of the tile; -1: none
+  };
+  const kvx_paged_select_args& a;
+  const Queries& q;
+  const int* table;
+  const uint16_t* bounds;
+  int lane, n, last;  // pages of the sequence, and those that are scored end here
+
+  __device__ __forceinline__ Scorer(const kvx_paged_select_args& a, const Queries& q, int b, int h, int n, int last)
+      : a(a), q(q), table(a.block_table + b * a.bt_stride_b), lane(threadIdx.x & 63), n(n), last(last) {
+    bounds = (const uint16_t*)a.bounds + h * a.b_stride_h + 8 * (lane >> 4);
+  }
+  // by all lanes of a workgroup of NT
+  template <int NT>
+  __device__ __forceinline__ static void put_queries(const kvx_paged_select_args& a, Queries& q, int b, int h) {
+    const int G = a.Hq / a.Hkv;
+    for (int i = threadIdx.x; i < 4 * HEADS * (D / 8); i += NT) {
+      const int g = i % (4 * HEADS), col = i / (4 * HEADS);
+      u32x4_t w = {0u, 0u, 0u, 0u};
+      if (g < G) w = *(const u32x4_t*)((const uint16_t*)a.q + b * a.q_stride_b + (int64_t)(h * G + g) * a.q_stride_h + 8 * col);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = j & 1 ? elem_hi<F16>(w[j >> 1]) : elem_lo<F16>(w[j >> 1]);
+        q[g >> 2][col >> 2][j][col & 3][g & 3] = f64x2_t{x > 0.0f ? x : 0.0f, x > 0.0f ? 0.0f : x};  // a NaN is the second's
+      }
+    }
+  }
+  __device__ __forceinline__ int entry(int first) const { return table[min(first + (lane & 15), n - 1)]; }
+  __device__ __forceinline__ void load(Tile& r, int entry, int first) const {
+    r.page = first + (lane & 15) < last && (uint32_t)entry < (uint32_t)a.num_pages ? entry : -1;
+    const uint16_t* at = bounds + (int64_t)max(r.page, 0) * a.b_stride_page;
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) {
+      r.lo[x] = *(const u32x4_t*)(at + 32 * x);
+      r.hi[x] = *(const u32x4_t*)(at + a.b_stride_side + 32 * x);
+    }
+  }
+  __device__ __forceinline__ void score(const Tile& r, int first, uint32_t* keys) const {
+    asm volatile("" ::: "memory");  // the queries are read anew, not held in registers, of which there are too few
+    const int kg = lane >> 4, G = a.Hq / a.Hkv;
+    double up[HEADS], down[HEADS];
+#pragma unroll
+    for (int f = 0; f < HEADS; ++f) up[f] = down[f] = 0.0;
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const double l = j & 1 ? elem_hi<F16>(r.lo[x][j >> 1]) : elem_lo<F16>(r.lo[x][j >> 1]), u = j & 1 ? elem_hi<F16>(r.hi[x][j >> 1]) : elem_lo<F16>(r.hi[x][j >> 1]);
+#pragma unroll
+        for (int f = 0; f < HEADS; ++f) {
+          const f64x2_t w = q[f][x][j][kg][lane & 3];
+          up[f] = __builtin_amdgcn_mfma_f64_4x4x4f64(u, w[0], up[f], 0, 0, 0);
+          down[f] = __builtin_amdgcn_mfma_f64_4x4x4f64(l, w[1], down[f], 0, 0, 0);
+        }
+      }
+    uint32_t key = kNever;
+#pragma unroll
+    for (int f = 0; f < HEADS; ++f)
+      if (4 * f + (lane & 3) < G) key = max(key, key_of(up[f] + down[f]));
+    key = max(key, (uint32_t)__builtin_amdgcn_mov_dpp((int)key, 0xB1, 0xf, 0xf, true));  // quad_perm [1,0,3,2]
+    key = max(key, (uint32_t)__builtin_amdgcn_mov_dpp((int)key, 0x4E, 0xf, 0xf, true));  // quad_perm [2,3,0,1]
+    const int mine = (lane & 12) + kg, i = first + mine;  // the page whose sums this lane has
+    const unsigned long long pages = __ballot(r.page >= 0);
+    if (!((pages >> mine) & 1)) key = kNever;
+    else if (i < a.first || i >= n - a.last) key = kAlways;
+    if ((lane & 3) == 0 && i < last) keys[i] = key;
+  }
+  // Pages first, first + each, ... below `last`, 16 at a time, with the next 16 on their way. A tile's entries of the table are read one tile ahead of its bounds, and before those of the
+  // tile in between: what waits for them waits for nothing else. Behind the last page, page 0 of the pool is read: loads under a condition would have to be waited for whether they
+  // are there or not. `ready`: what has to be done before the queries are read
+  template <typename F>
+  __device__ __forceinline__ void run(int first, int each, uint32_t* keys, F ready) const {
+    int next = entry(first), then = entry(first + each);
+    Tile one, two;
+    load(one, next, first);
+    ready();
+    for (; first < last; first += 2 * each) {
+      next = entry(first + 2 * each);
+      __builtin_amdgcn_sched_barrier(0);
+      load(two, then, first + each);
+      __builtin_amdgcn_sched_barrier(0);
+      score(one, first, keys);
+      if (first + each >= last) break;
+      __builtin_amdgcn_sched_barrier(0);
+      then = entry(first + 3 * each);
+      __builtin_amdgcn_sched_barrier(0);
+      load(one, next, first + 2 * each);
+      __builtin_amdgcn_sched_barrier(0);
+      score(two, first + each, keys);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+
 constexpr int score_workgroups(int D) { return D == 256 ? 2 : 4; }  // a compute unit: what registers leave room for
 template <int D, bool F16, int HEADS /* of the group, in fours */>
 __global__ __launch_bounds__(NTHREADS, score_workgroups(D)) void select_score_kernel(const SelectParams p) {
-  typedef double f64x2_t __attribute__((ext_vector_type(2)));
+  typedef Scorer<D, F16, HEADS> S;
   const kvx_paged_select_args& a = p.a;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = lane >> 4, B = a.B, Hkv = a.Hkv, G = a.Hq / Hkv;
-  __shared__ __align__(16) f64x2_t qs[HEADS][D / 32][8][4][4];  // value 32 x + 8 kg + j of head 4 f + g at [f][x][j][kg][g]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), B = a.B, Hkv = a.Hkv;
+  __shared__ __align__(16) typename S::Queries qs;
 
   // ---- this workgroup's units: every wavefront finds them for itself, 64 sequences at a time
   const int windows = (B + 63) / 64;
@@ -275,89 +377,16 @@ __global__ __launch_bounds__(NTHREADS, score_workgroups(D)) void select_score_ke
     before = __builtin_amdgcn_readlane(upto, 63);
   }
 
-  struct Tile {
-    u32x4_t lo[D / 32], hi[D / 32];
-    int page;  // of the pool, of page lane % 16 of the tile; -1: none
-  };
   for (bool again = false;; again = true) {
     const int n = __builtin_amdgcn_readlane(lane_pages, b & 63), units = units_in(n);
     if (units > 0) {
       const int h = (unit - begin_b) / units, from = unit - begin_b - h * units, count = min(units - from, end - unit), pair = b * Hkv + h;
-      const int last = min(n, (from + count) * UNIT);
-      const int* table = a.block_table + b * a.bt_stride_b;
-      const uint16_t* bounds = (const uint16_t*)a.bounds + h * a.b_stride_h + 8 * kg;
-      auto entry = [&](int first) { return table[min(first + (lane & 15), n - 1)]; };
-      auto load = [&](Tile& r, int entry, int first) {
-        r.page = first + (lane & 15) < last && (uint32_t)entry < (uint32_t)a.num_pages ? entry : -1;
-        const uint16_t* at = bounds + (int64_t)max(r.page, 0) * a.b_stride_page;
-#pragma unroll
-        for (int x = 0; x < D / 32; ++x) {
-          r.lo[x] = *(const u32x4_t*)(at + 32 * x);
-          r.hi[x] = *(const u32x4_t*)(at + a.b_stride_side + 32 * x);
-        }
-      };
-      auto score = [&](const Tile& r, int first) {
-        asm volatile("" ::: "memory");  // the queries are read anew, not held in registers, of which there are too few
-        double up[HEADS], down[HEADS];
-#pragma unroll
-        for (int f = 0; f < HEADS; ++f) up[f] = down[f] = 0.0;
-#pragma unroll
-        for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const double l = j & 1 ? elem_hi<F16>(r.lo[x][j >> 1]) : elem_lo<F16>(r.lo[x][j >> 1]), u = j & 1 ? elem_hi<F16>(r.hi[x][j >> 1]) : elem_lo<F16>(r.hi[x][j >> 1]);
-#pragma unroll
-            for (int f = 0; f < HEADS; ++f) {
-              const f64x2_t q = qs[f][x][j][kg][lane & 3];
-              up[f] = __builtin_amdgcn_mfma_f64_4x4x4f64(u, q[0], up[f], 0, 0, 0);
-              down[f] = __builtin_amdgcn_mfma_f64_4x4x4f64(l, q[1], down[f], 0, 0, 0);
-            }
-          }
-        uint32_t key = kNever;
-#pragma unroll
-        for (int f = 0; f < HEADS; ++f)
-          if (4 * f + (lane & 3) < G) key = max(key, key_of(up[f] + down[f]));
-        key = max(key, (uint32_t)__builtin_amdgcn_mov_dpp((int)key, 0xB1, 0xf, 0xf, true));  // quad_perm [1,0,3,2]
-        key = max(key, (uint32_t)__builtin_amdgcn_mov_dpp((int)key, 0x4E, 0xf, 0xf, true));  // quad_perm [2,3,0,1]
-        const int mine = (lane & 12) + kg, i = first + mine;  // the page whose sums this lane has
-        const unsigned long long pages = __ballot(r.page >= 0);
-        if (!((pages >> mine) & 1)) key = kNever;
-        else if (i < a.first || i >= n - a.last) key = kAlways;
-        if ((lane & 3) == 0 && i < last) p.keys[(int64_t)pair * a.max_pages + i] = key;
-      };
-      // A tile's entries of the table are read one tile ahead of its bounds, and before those of the tile in between: what waits for them waits for nothing else. Behind the
-      // last page, page 0 of the pool is read: loads under a condition would have to be waited for whether they are there or not.
-      int first = from * UNIT + wave * 16;
-      int next = entry(first), then = entry(first + UNIT);
-      Tile one, two;
-      if (again) __syncthreads();  // the queries before are read
-      for (int i = threadIdx.x; i < 4 * HEADS * (D / 8); i += NTHREADS) {
-        const int g = i % (4 * HEADS), col = i / (4 * HEADS);
-        u32x4_t q = {0u, 0u, 0u, 0u};
-        if (g < G) q = *(const u32x4_t*)((const uint16_t*)a.q + b * a.q_stride_b + (int64_t)(h * G + g) * a.q_stride_h + 8 * col);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float x = j & 1 ? elem_hi<F16>(q[j >> 1]) : elem_lo<F16>(q[j >> 1]);
-          qs[g >> 2][col >> 2][j][col & 3][g & 3] = f64x2_t{x > 0.0f ? x : 0.0f, x > 0.0f ? 0.0f : x};  // a NaN is the second's
-        }
-      }
-      load(one, next, first);
-      __syncthreads();
-      for (; first < last; first += 2 * UNIT) {
-        next = entry(first + 2 * UNIT);
-        __builtin_amdgcn_sched_barrier(0);
-        load(two, then, first + UNIT);
-        __builtin_amdgcn_sched_barrier(0);
-        score(one, first);
-        if (first + UNIT >= last) break;
-        __builtin_amdgcn_sched_barrier(0);
-        then = entry(first + 3 * UNIT);
-        __builtin_amdgcn_sched_barrier(0);
-        load(one, next, first + 2 * UNIT);
-        __builtin_amdgcn_sched_barrier(0);
-        score(two, first + UNIT);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      const S s(a, qs, b, h, n, min(n, (from + count) * UNIT));
+      s.run(from * UNIT + wave * 16, UNIT, p.keys + (int64_t)pair * a.max_pages, [&] {
+        if (again) __syncthreads();  // the queries before are read
+        S::template put_queries<NTHREADS>(a, qs, b, h);
+        __syncthreads();
+      });
       unit += count;
       if (unit >= end) break;
     }
@@ -367,6 +396,54 @@ __global__ __launch_bounds__(NTHREADS, score_workgroups(D)) void select_score_ke
       if ((b & 63) == 0 && b < B) lane_pages = window(b >> 6);
     }
   }
+}
+
+// Scores and choice in one launch, a workgroup for a (sequence, KV head) of up to 128 pages: 16 a wavefront, whose keys meet in LDS, where each is compared with all others.
+// 64 pages, 32 / 8 heads of 128: 1 sequence 6.5 us, in two launches 5.4 and 3.8 and what lies between, 32 sequences 6.7, 5.6 and 4.2, 128 16.0, 12.6 and 5.6. With more pages a
+// workgroup that has them alone takes longer: 512 pages, 1 sequence, 13.6, 5.5 and 4.1.
+constexpr int FEW = 128;
+template <int D, bool F16, int HEADS>
+__global__ __launch_bounds__(4 * FEW) void select_few_kernel(const SelectParams p) {
+  typedef Scorer<D, F16, HEADS> S;
+  const kvx_paged_select_args& a = p.a;
+  __shared__ __align__(16) typename S::Queries qs;
+  __shared__ __align__(16) uint32_t keys[FEW];
+  __shared__ int taken[FEW / 16];
+  const int pair = blockIdx.x, b = pair / a.Hkv, h = pair - b * a.Hkv, n = pages_of_sequence(a, b), tid = threadIdx.x, lane = tid & 63;
+  if (tid < FEW) keys[tid] = kNever;
+  if (n > 0) {
+    const S s(a, qs, b, h, n, n);
+    s.run(16 * __builtin_amdgcn_readfirstlane(tid >> 6), FEW, keys, [&] {
+      S::template put_queries<4 * FEW>(a, qs, b, h);
+      __syncthreads();
+    });
+  }
+  __syncthreads();
+  // four lanes a key, each of which compares it with a quarter of the others
+  const int i = tid >> 2, part = tid & 3;
+  const uint32_t key = keys[i];
+  int before = 0;  // keys that come first
+#pragma unroll
+  for (int j = 0; j < FEW / 4; j += 4) {
+    const u32x4_t x = *(const u32x4_t*)(keys + FEW / 4 * part + j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) before += x[e] + (FEW / 4 * part + j + e < i) > key;  // of equal ones those in front; no key is the largest of all words
+  }
+  before += __builtin_amdgcn_mov_dpp(before, 0xB1, 0xf, 0xf, true);  // quad_perm [1,0,3,2]
+  before += __builtin_amdgcn_mov_dpp(before, 0x4E, 0xf, 0xf, true);  // quad_perm [2,3,0,1]
+  const bool take = key != kNever && before < a.count;
+  const unsigned long long m = __ballot(take && part == 0);
+  if (lane == 0) taken[tid >> 6] = __popcll(m);
+  __syncthreads();
+  int to = __popcll(m & ((1ull << lane) - 1)), all = 0;
+#pragma unroll
+  for (int w = 0; w < FEW / 16; ++w) {
+    to += w < tid >> 6 ? taken[w] : 0;
+    all += taken[w];
+  }
+  int32_t* out = a.chosen + (int64_t)pair * a.count;
+  if (take && part == 0) out[to] = i;
+  for (int j = all + tid; j < a.count; j += 4 * FEW) out[j] = -1;
 }
 
 // The `count` largest keys of a (sequence, KV head), of equal ones the first, in order of their pages, for up to R * NT pages, whose keys stay in registers. The last key that is taken lies
@@ -611,7 +688,7 @@ int launch_paged_bounds(const kvx_paged_bounds_args& a, hipStream_t st) {
   return KVX_OK;
 }
 
-size_t paged_select_workspace(const kvx_paged_select_args& a) { return (size_t)4 * a.B * a.Hkv * a.max_pages; }
+size_t paged_select_workspace(const kvx_paged_select_args& a) { return a.max_pages <= FEW ? 0 : (size_t)4 * a.B * a.Hkv * a.max_pages; }
 
 int launch_paged_select(const kvx_paged_select_args& a, hipStream_t st) {
   const SelectParams p = {a, (uint32_t*)a.workspace};
@@ -620,9 +697,12 @@ int launch_paged_select(const kvx_paged_select_args& a, hipStream_t st) {
               a.Hkv);
   const unsigned blocks = (unsigned)min(units, (int64_t)score_workgroups(a.D) * num_cus());
   const int group = a.Hq / a.Hkv;
+  const bool few = a.max_pages <= FEW;
   auto go = [&](auto d, auto f16) {
     auto score = [&](auto heads) {
-      hipLaunchKernelGGL((select_score_kernel<decltype(d)::value, decltype(f16)::value, decltype(heads)::value>), dim3(blocks), dim3(NTHREADS), 0, st, p);
+      constexpr int D = decltype(d)::value, HEADS = decltype(heads)::value;
+      if (few) hipLaunchKernelGGL((select_few_kernel<D, decltype(f16)::value, HEADS>), dim3((unsigned)count), dim3(4 * FEW), 0, st, p);
+      else hipLaunchKernelGGL((select_score_kernel<D, decltype(f16)::value, HEADS>), dim3(blocks), dim3(NTHREADS), 0, st, p);
     };
     if (group <= 4) score(std::integral_constant<int, 1>{});
     else if (group <= 8) score(std::integral_constant<int, 2>{});
@@ -635,21 +715,25 @@ int launch_paged_select(const kvx_paged_select_args& a, hipStream_t st) {
   if (a.D == 256) go_type(std::integral_constant<int, 256>{});
   else if (a.D == 128) go_type(std::integral_constant<int, 128>{});
   else go_type(std::integral_constant<int, 64>{});
-  const dim3 pairs((unsigned)(a.B * a.Hkv));
+  if (few) {
+    KVX_HIP(hipGetLastError());
+    return KVX_OK;
+  }
+  const dim3 pairs((unsigned)count);
   // 512 lanes take less time than 1024 up to 2048 pages, as long at 4096, and more beyond: 1024 pages 4.2 and 5.0 us, 4096 5.9 and 5.9, 8192 7.0 and 6.7
   auto choose = [&](auto r, auto nt) {
     constexpr int R = decltype(r)::value, NT = decltype(nt)::value;
     hipLaunchKernelGGL((select_choose_kernel<R, NT>), pairs, dim3(NT), 0, st, p);
   };
-  const std::integral_constant<int, 512> few;
-  const std::integral_constant<int, 1024> many;
-  if (a.max_pages <= 512) choose(std::integral_constant<int, 1>{}, few);
-  else if (a.max_pages <= 1024) choose(std::integral_constant<int, 2>{}, few);
-  else if (a.max_pages <= 2048) choose(std::integral_constant<int, 4>{}, few);
-  else if (a.max_pages <= 4096) choose(std::integral_constant<int, 4>{}, many);
-  else if (a.max_pages <= 8192) choose(std::integral_constant<int, 8>{}, many);
-  else if (a.max_pages <= 16384) choose(std::integral_constant<int, 16>{}, many);
-  else if (a.max_pages <= 32768) choose(std::integral_constant<int, 32>{}, many);
+  const std::integral_constant<int, 512> half;
+  const std::integral_constant<int, 1024> whole;
+  if (a.max_pages <= 512) choose(std::integral_constant<int, 1>{}, half);
+  else if (a.max_pages <= 1024) choose(std::integral_constant<int, 2>{}, half);
+  else if (a.max_pages <= 2048) choose(std::integral_constant<int, 4>{}, half);
+  else if (a.max_pages <= 4096) choose(std::integral_constant<int, 4>{}, whole);
+  else if (a.max_pages <= 8192) choose(std::integral_constant<int, 8>{}, whole);
+  else if (a.max_pages <= 16384) choose(std::integral_constant<int, 16>{}, whole);
+  else if (a.max_pages <= 32768) choose(std::integral_constant<int, 32>{}, whole);
   else hipLaunchKernelGGL(select_choose_long_kernel, pairs, dim3(CHOOSERS), 0, st, p);
   KVX_HIP(hipGetLastError());
   return KVX_OK;

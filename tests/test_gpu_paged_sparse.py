@@ -301,11 +301,41 @@ def test_select_of_batches(gpu, B, Hkv, low, high):
         choose_and_check(*args, 16, count, 1, 2)
 
 
+@pytest.mark.parametrize("width", [1, 2, 16, 17, 127, 128, 129, 512, 513, 1024, 1025, 2048, 2049, 4096, 4097, 8192, 8193, 16384, 16385, 32768, 32769])
+def test_select_of_table_widths(gpu, width):
+    """Where one kernel's pages end and the next one's begin."""
+    print("select", width, flush=True)
+    for Hq, Hkv, D, dtype in ((8, 2, 128, torch.bfloat16), (5, 1, 64, torch.float16), (32, 2, 256, torch.bfloat16)):
+        if D == 256 and width > 2049:
+            continue
+        args = a_choice(gpu, [16 * width, 0, 16 * width - 5, 8 * width + 3, 1], Hq, Hkv, D, 16, dtype, seed=width, width=width)
+        for count, first, last in ((1, 0, 1), (min(40, width + 3), 1, 0), (max(2, width // 2), 1, 1), (width, 0, 0)):
+            choose_and_check(*args, 16, count, first, last)
+
+
 def test_select_of_very_long_sequences(gpu):
     """More pages than a workgroup holds: 70000 of 16 tokens."""
     args = a_choice(gpu, [1120000, 5, 530000], 2, 1, 64, 16, seed=2)
     for count in (64, 40000):
         choose_and_check(*args, 16, count)
+
+
+@pytest.mark.parametrize("pages", [100, 128])
+@pytest.mark.parametrize("group", [1, 5, 16])
+def test_select_of_few_pages(gpu, group, pages):
+    """Tables that one workgroup has whole: ties, what is not finite, pages that are not there."""
+    q, bounds, table, lens = a_choice(gpu, [16 * pages, 500, 7, 1024], 2 * group, 2, 128, 16, seed=group, width=pages)
+    choose_and_check(q, bounds, table, lens, 16, 20, 1, 2)
+    bounds[int(table[0, 40]), 1, 0, 3] = math.nan
+    bounds[int(table[0, 41]), :, 1, 3] = math.inf
+    table[0, ::3], table[1, 5], table[3, :] = -1, bounds.shape[0], -7
+    got = choose_and_check(q, bounds, table, lens, 16, 12, 2, 3)
+    assert 40 in got[0, 1].tolist() and 41 in got[0, 0].tolist() and (got[3] == -1).all()
+    q[1, 0, 0] = math.inf
+    choose_and_check(q, bounds, table, lens, 16, 60, 0, 0)
+    bounds[:] = bounds[3:4].clone()
+    choose_and_check(q, bounds, table, lens, 16, 9, 0, 1)
+    choose_and_check(torch.zeros_like(q), bounds, table, lens, 16, 50, 0, 0)
 
 
 @pytest.mark.parametrize("group", [1, 4, 7, 16])
@@ -517,6 +547,17 @@ def test_chosen_of_batches(gpu, store, B, Hq, Hkv, D, page, low, high, count):
     lens = [high] + torch.randint(low, high + 1, (B - 1,), generator=gen).tolist()
     pool = Pool(gpu, store, lens, Hkv, D, page, seed=B + 1, width=-(-high // page) + 20)
     attend_and_check(pool, gpu, Hq, some_pages(pool, count, seed=B))
+
+
+@pytest.mark.parametrize("store", STORES)
+@pytest.mark.parametrize("D,page,count", [(128, 16, 64), (64, 64, 9), (256, 128, 16)])
+def test_chosen_of_many_lists(gpu, store, D, page, count):
+    """Lists enough to keep all units busy, each a workgroup's; of 512 tokens more and to 2048, full and not."""
+    gen = torch.Generator().manual_seed(D)
+    lens = torch.randint(0, 70, (140,), generator=gen).tolist()
+    lens[3], lens[5], lens[17], lens[70], lens[138], lens[139] = 0, count * page + 1, count * page, 1, count * page // 2 + 9, 2 * count * page
+    pool = Pool(gpu, store, lens, 4, D, page, seed=count)
+    attend_and_check(pool, gpu, 8, some_pages(pool, count, seed=count))
 
 
 @pytest.mark.parametrize("store,D,page", [("bf16", 64, 16), ("u8_fp16", 128, 64), ("u4", 64, 32), ("u4_fp16", 256, 16)])
