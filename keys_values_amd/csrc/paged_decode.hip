@@ -71,6 +71,7 @@ struct ChosenParams : PagedParams {
   const int* chosen;
   int64_t ch_sb, ch_sh;
   int table_cap;  // tokens of a table's pages
+  int whole;      // a unit is a list's, so that nothing has to be known of the lengths to find a workgroup's
 };
 
 // Keys that a pair of a sequence of `len` tokens goes through: its tokens, or the places of the pages that are chosen
@@ -254,11 +255,14 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
   auto window = [&](int i) { return 64 * i + lane < B ? p.lens[64 * i + lane] : -1; };
   auto units_in = [&](int len, int i) { return 64 * i + lane < B ? units_of(len, p, extra) : 0; };
   int lane_len = 0, mine = 0;  // lane_len: of sequence (b & ~63) + lane
-  for (int i = 0; i < windows; ++i) {
-    lane_len = window(i);
-    mine += units_in(lane_len, i);
-  }
-  const int total = __builtin_amdgcn_readlane(scan(mine), 63) * Hkv;
+  bool whole = false;
+  if constexpr (CHOSEN) whole = p.whole;
+  if (!whole)
+    for (int i = 0; i < windows; ++i) {
+      lane_len = window(i);
+      mine += units_in(lane_len, i);
+    }
+  const int total = whole ? B * Hkv : __builtin_amdgcn_readlane(scan(mine), 63) * Hkv;
   // Workgroups that share the units, of the grid's two or three a compute unit: all where pairs are short (of up to four units on average; B256, 32 / 8 heads of 128, 50 to 400
   // tokens: 42.7 us, 44.4 with two a compute unit, 54.2 with one), two elsewhere (64 sequences of 1 to 8192, 28 / 4 heads: 30.9, 33.3 with one, 32.1 with three), and
   // one, whose partials are the fewest, where pairs are long and rows of 128 bytes and more keep enough of them on their way (16 x 16384, plain rows of 128: 158.3, 162.0
@@ -271,7 +275,12 @@ __global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged
   if (tid == 0 && p.part_of && !p.by_pair) p.part_of[2 * w + 1] = 0;
   if (unit >= end) return;
   int b, begin_b;  // its sequence, and the sequence's first unit
-  for (int i = 0, before = 0;; ++i) {
+  if (whole) {
+    b = unit / Hkv;
+    begin_b = b * Hkv;
+    lane_len = window(b >> 6);
+  }
+  for (int i = 0, before = 0; !whole; ++i) {
     if (windows > 1) lane_len = window(i);
     mine = units_in(lane_len, i);
     const int upto = before + scan(mine);
@@ -804,6 +813,8 @@ __global__ __launch_bounds__(NT) void paged_join_kernel(const PagedParams p) {
   if (p.lse && d == 0) p.lse[(int64_t)pair * p.Gr + g] = sum == 0.0f ? -INFINITY : all + fast_log2(sum);
 }
 
+bool splits(const PagedParams& p) { return p.cap > (1 << p.unit); }
+
 ChosenParams params_of(const kvx_paged_decode_args& a, const kvx_chosen_pages* c) {
   const kvx_pages& g = a.pages;
   const bool plain = kv_is_plain(g.kv_dtype);
@@ -856,10 +867,11 @@ ChosenParams params_of(const kvx_paged_decode_args& a, const kvx_chosen_pages* c
   // sequences, plain, 16.6 and 19.8. Where most sequences have few tokens the longest list takes longer than it would in parts (1024 plain keys 20 us, 13 and 4 in parts).
   const int64_t lists = (int64_t)a.B * g.Hkv;
   if (c && p.cap > 4 * UNIT && p.cap <= 2048 && 4 * lists >= p.cap) p.unit = 32 - __builtin_clz(p.cap - 1);
+  p.whole = !splits(p);
   // Beginning a pair of codes takes the time of one unit of 8-bit rows, or two of 4-bit ones: it counts as such, or the workgroups that get the short pairs come last. 92
   // sequences of lengths even in the logarithm from 15 to 9560, 4-bit rows of 128, 32 / 4 heads: 40.8 us without, 29.6 with one unit, 26.2 with two; 14 from 25 to 35609, 8-bit
   // rows of 256: 76.8 without, 63.1 with one or two. Plain rows, whose units take longer, only lose: 200 of 1 to 3000, 65.8 without, 68.5 with one.
-  p.extra = plain || p.unit == 9 ? 0 : kv_is_u4(g.kv_dtype) ? 2 : 1;
+  p.extra = plain || !splits(p) ? 0 : kv_is_u4(g.kv_dtype) ? 2 : 1;
   p.cus = num_cus();
   // One workgroup a compute unit for the only pair: the partials of more take longer to join than they save (one of 100000 tokens, 16 heads of 128: 21.7 us, 33.8
   // with three).
@@ -870,7 +882,6 @@ ChosenParams params_of(const kvx_paged_decode_args& a, const kvx_chosen_pages* c
   p.by_pair = pairs <= p.workgroups;
   return p;
 }
-bool splits(const PagedParams& p) { return p.cap > (1 << p.unit); }
 
 template <int D>
 void launch_head(const ChosenParams& p, int kv_dtype, hipStream_t st) {

@@ -223,11 +223,9 @@ __device__ __forceinline__ uint32_t key_of(double sum) {
 struct SelectParams {
   kvx_paged_select_args a;
   uint32_t* keys;  // (B, Hkv, max_pages)
+  int shift;       // log2 of the page size
+  __device__ __forceinline__ int pages(int b) const { return (min(max(a.lens[b], 0), a.max_pages << shift) + a.page_size - 1) >> shift; }  // of a sequence
 };
-__device__ __forceinline__ int pages_of_sequence(const kvx_paged_select_args& a, int b) {
-  const int len = max(a.lens[b], 0);
-  return (int)min(((int64_t)len + a.page_size - 1) / a.page_size, (int64_t)a.max_pages);
-}
 
 // v_mfma_f64_4x4x4, four blocks of 4 pages, 4 heads and 4 values: lane l has a value of page l % 16 (A), of head l % 4 (B), and gets the sum of page
 // 4 (l / 4 % 4) + l / 16 and head l % 4. Products of 16-bit values are exact in 32 bits, and their sums, in 64, differ with the order by less than what the rounding to 32 sees.
@@ -259,22 +257,34 @@ struct Scorer {
       : a(a), q(q), table(a.block_table + b * a.bt_stride_b), lane(threadIdx.x & 63), n(n), last(last) {
     bounds = (const uint16_t*)a.bounds + h * a.b_stride_h + 8 * (lane >> 4);
   }
-  // by all lanes of a workgroup of NT
+  // The queries to LDS, by all lanes of a workgroup of NT: on their way from construction on, so that what a wavefront waits for before `put` is theirs and not the bounds'
   template <int NT>
-  __device__ __forceinline__ static void put_queries(const kvx_paged_select_args& a, Queries& q, int b, int h) {
-    const int G = a.Hq / a.Hkv;
-    for (int i = threadIdx.x; i < 4 * HEADS * (D / 8); i += NT) {
-      const int g = i % (4 * HEADS), col = i / (4 * HEADS);
-      u32x4_t w = {0u, 0u, 0u, 0u};
-      if (g < G) w = *(const u32x4_t*)((const uint16_t*)a.q + b * a.q_stride_b + (int64_t)(h * G + g) * a.q_stride_h + 8 * col);
+  struct Fetch {
+    static constexpr int ALL = 4 * HEADS * (D / 8), EACH = (ALL + NT - 1) / NT;
+    u32x4_t w[EACH];
+    __device__ __forceinline__ Fetch(const kvx_paged_select_args& a, int b, int h) {
+      const int G = a.Hq / a.Hkv;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = j & 1 ? elem_hi<F16>(w[j >> 1]) : elem_lo<F16>(w[j >> 1]);
-        q[g >> 2][col >> 2][j][col & 3][g & 3] = f64x2_t{x > 0.0f ? x : 0.0f, x > 0.0f ? 0.0f : x};  // a NaN is the second's
+      for (int e = 0; e < EACH; ++e) {
+        const int i = min((int)threadIdx.x + e * NT, ALL - 1), g = i % (4 * HEADS), col = i / (4 * HEADS);
+        w[e] = *(const u32x4_t*)((const uint16_t*)a.q + b * a.q_stride_b + (int64_t)(h * G + min(g, G - 1)) * a.q_stride_h + 8 * col);
       }
     }
-  }
-  __device__ __forceinline__ int entry(int first) const { return table[min(first + (lane & 15), n - 1)]; }
+    __device__ __forceinline__ void put(Queries& q) const {  // heads behind the group's last: copies of it, whose sums nobody looks at
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int i = threadIdx.x + e * NT, g = i % (4 * HEADS), col = i / (4 * HEADS);
+        if (i < ALL) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float x = j & 1 ? elem_hi<F16>(w[e][j >> 1]) : elem_lo<F16>(w[e][j >> 1]);
+            q[g >> 2][col >> 2][j][col & 3][g & 3] = f64x2_t{x > 0.0f ? x : 0.0f, x > 0.0f ? 0.0f : x};  // a NaN is the second's
+          }
+        }
+      }
+    }
+  };
+  __device__ __forceinline__ int entry(int first) const { return table[min(first + (lane & 15), a.max_pages - 1)]; }  // does not wait for n
   __device__ __forceinline__ void load(Tile& r, int entry, int first) const {
     r.page = first + (lane & 15) < last && (uint32_t)entry < (uint32_t)a.num_pages ? entry : -1;
     const uint16_t* at = bounds + (int64_t)max(r.page, 0) * a.b_stride_page;
@@ -322,6 +332,7 @@ struct Scorer {
     int next = entry(first), then = entry(first + each);
     Tile one, two;
     load(one, next, first);
+    __builtin_amdgcn_sched_barrier(0);
     ready();
     for (; first < last; first += 2 * each) {
       next = entry(first + 2 * each);
@@ -351,7 +362,7 @@ __global__ __launch_bounds__(NTHREADS, score_workgroups(D)) void select_score_ke
 
   // ---- this workgroup's units: every wavefront finds them for itself, 64 sequences at a time
   const int windows = (B + 63) / 64;
-  auto window = [&](int i) { return 64 * i + lane < B ? pages_of_sequence(a, 64 * i + lane) : 0; };
+  auto window = [&](int i) { return 64 * i + lane < B ? p.pages(64 * i + lane) : 0; };
   auto units_in = [&](int pages) { return (pages + UNIT - 1) / UNIT; };
   int lane_pages = 0, mine = 0;  // lane_pages: of sequence (b & ~63) + lane
   for (int i = 0; i < windows; ++i) {
@@ -381,10 +392,11 @@ __global__ __launch_bounds__(NTHREADS, score_workgroups(D)) void select_score_ke
     const int n = __builtin_amdgcn_readlane(lane_pages, b & 63), units = units_in(n);
     if (units > 0) {
       const int h = (unit - begin_b) / units, from = unit - begin_b - h * units, count = min(units - from, end - unit), pair = b * Hkv + h;
+      const typename S::template Fetch<NTHREADS> queries(a, b, h);
       const S s(a, qs, b, h, n, min(n, (from + count) * UNIT));
       s.run(from * UNIT + wave * 16, UNIT, p.keys + (int64_t)pair * a.max_pages, [&] {
         if (again) __syncthreads();  // the queries before are read
-        S::template put_queries<NTHREADS>(a, qs, b, h);
+        queries.put(qs);
         __syncthreads();
       });
       unit += count;
@@ -409,15 +421,18 @@ __global__ __launch_bounds__(4 * FEW) void select_few_kernel(const SelectParams 
   __shared__ __align__(16) typename S::Queries qs;
   __shared__ __align__(16) uint32_t keys[FEW];
   __shared__ int taken[FEW / 16];
-  const int pair = blockIdx.x, b = pair / a.Hkv, h = pair - b * a.Hkv, n = pages_of_sequence(a, b), tid = threadIdx.x, lane = tid & 63;
+  const int pair = blockIdx.x, b = pair / a.Hkv, h = pair - b * a.Hkv, tid = threadIdx.x, lane = tid & 63;
+  const typename S::template Fetch<4 * FEW> queries(a, b, h);
+  const int n = p.pages(b);
   if (tid < FEW) keys[tid] = kNever;
-  if (n > 0) {
-    const S s(a, qs, b, h, n, n);
-    s.run(16 * __builtin_amdgcn_readfirstlane(tid >> 6), FEW, keys, [&] {
-      S::template put_queries<4 * FEW>(a, qs, b, h);
-      __syncthreads();
-    });
-  }
+  const S s(a, qs, b, h, n, n);
+  const int first = 16 * __builtin_amdgcn_readfirstlane(tid >> 6);
+  auto ready = [&] {
+    queries.put(qs);
+    __syncthreads();
+  };
+  if (first < n) s.run(first, FEW, keys, ready);
+  else ready();
   __syncthreads();
   // four lanes a key, each of which compares it with a quarter of the others
   const int i = tid >> 2, part = tid & 3;
@@ -453,7 +468,7 @@ template <int R, int NT>
 __global__ __launch_bounds__(NT) void select_choose_kernel(const SelectParams p) {
   constexpr int BINS = 2048, WAVES = NT / 64, EACH = BINS / NT;  // EACH: parts a lane counts up, from the largest down
   const kvx_paged_select_args& a = p.a;
-  const int pair = blockIdx.x, b = pair / a.Hkv, n = pages_of_sequence(a, b), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int pair = blockIdx.x, b = pair / a.Hkv, n = p.pages(b), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   __shared__ int counts[BINS], sums[WAVES], at_bin, at_rest, at_count;
   __shared__ uint32_t lows[WAVES], highs[WAVES];
   __shared__ int places[R * WAVES];
@@ -461,7 +476,9 @@ __global__ __launch_bounds__(NT) void select_choose_kernel(const SelectParams p)
   int32_t* out = a.chosen + (int64_t)pair * a.count;
   uint32_t key[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) key[r] = r * NT + tid < n ? keys[r * NT + tid] : kNever;
+  for (int r = 0; r < R; ++r) key[r] = keys[min(r * NT + tid, a.max_pages - 1)];  // does not wait for n
+#pragma unroll
+  for (int r = 0; r < R; ++r) key[r] = r * NT + tid < n ? key[r] : kNever;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) counts[NT * e + tid] = 0;
   // ---- range of the keys that are neither taken anyway nor left out, and the numbers of those (in both halves of a word of their own: n < 2^26)
@@ -590,7 +607,7 @@ __global__ __launch_bounds__(NT) void select_choose_kernel(const SelectParams p)
 constexpr int CHOOSERS = 1024;
 __global__ __launch_bounds__(CHOOSERS) void select_choose_long_kernel(const SelectParams p) {
   const kvx_paged_select_args& a = p.a;
-  const int pair = blockIdx.x, b = pair / a.Hkv, n = pages_of_sequence(a, b), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int pair = blockIdx.x, b = pair / a.Hkv, n = p.pages(b), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   constexpr int WAVES = CHOOSERS / 64, BINS = 2048;
   __shared__ int counts[BINS], sums[WAVES], at_bin, at_rest;
   const uint32_t* keys = p.keys + (int64_t)pair * a.max_pages;
@@ -691,7 +708,7 @@ int launch_paged_bounds(const kvx_paged_bounds_args& a, hipStream_t st) {
 size_t paged_select_workspace(const kvx_paged_select_args& a) { return a.max_pages <= FEW ? 0 : (size_t)4 * a.B * a.Hkv * a.max_pages; }
 
 int launch_paged_select(const kvx_paged_select_args& a, hipStream_t st) {
-  const SelectParams p = {a, (uint32_t*)a.workspace};
+  const SelectParams p = {a, (uint32_t*)a.workspace, __builtin_ctz(a.page_size)};
   const int64_t count = (int64_t)a.B * a.Hkv, units = count * ((a.max_pages + UNIT - 1) / UNIT);
   KVX_REQUIRE(count < (1 << 21) && units < (1 << 30), KVX_ERR_UNSUPPORTED, "kvx_paged_select: %d sequences of up to %d pages, %d KV heads in one call", a.B, a.max_pages,
               a.Hkv);
