@@ -581,7 +581,7 @@ size_t kvx_paged_decode_workspace_bytes(const kvx_paged_decode_args* args);
  * the value heads are too (rotary.qkv holds all of them; its key and value heads are left as they are). To the bit what the two calls store. A token whose
  * position is negative or behind the tables' last row is padding: nothing of it is changed or stored, whatever its slot. One without a slot has its queries turned.
  * Two tokens of one call with the same slot: one of them is stored, or parts of each. rotary's Hkv, D and elem_dtype have to fit the pages. A call takes fewer than
- * 2^23 groups of 2048 / D heads: of tokens * Hq queries and tokens * Hkv plain rows, of codes Hkv times the groups of tokens. */
+ * 2^23 workgroups: one a token, or, of up to two tokens a compute unit, one for 2048 / D of its heads; and of codes Hkv times one for 2048 / D tokens. */
 typedef struct kvx_paged_append_args {
   kvx_rotary_args rotary;
   kvx_pages pages;
@@ -593,7 +593,7 @@ int kvx_paged_append(const kvx_paged_append_args* args, void* stream);
  * the lowest and the highest of the page's keys among these lens[b], value by value, to bounds[page * b_stride_page + h * b_stride_h + d] and, b_stride_side further,
  * of the store's element type. Rows of codes count as kvx_paged_read gives them. A NaN among a page's values makes its bounds NaN. Bounds of other pages, and of pages
  * that the pool does not have, are left as they are. A page of two sequences gets the bounds of one of them: share pages that are full, or have as many tokens in
- * both. pages.v and the state of V are not read, but checked. lens and the table are read on the device alone. A call looks at fewer than 2^22 (sequence,
+ * both. pages.v and the state of V are not read, but checked. lens and the table are read on the device alone. A call looks at fewer than 2^30 (sequence,
  * page, KV head), shorter sequences counted as the longest that the table and `tokens` allow. */
 typedef struct kvx_paged_bounds_args {
   kvx_pages pages;
@@ -608,10 +608,11 @@ int kvx_paged_bounds(const kvx_paged_bounds_args* args, void* stream);
 
 /* The pages that a query attends to. A page of a sequence (the i-th, i < ceil(lens[b] / page_size) and max_pages) has for KV head h the score
  *   max over the query heads of h of sum_d max(q[d] * low[d], q[d] * high[d]),
- * which is no less than any of its keys' products with them. Sums are formed in 64 bits and rounded to 32; a score that is not finite counts as infinite. Of every (sequence, KV head)
+ * which, with bounds as kvx_paged_bounds leaves them (low <= high), is no less than any of its keys' products with them. Sums are formed in 64 bits and rounded to 32; a score that is
+ * not finite, or of bounds or queries that are not, counts as infinite. Of every (sequence, KV head)
  * the first `first` and the last `last` pages are chosen, and the others by their scores, of equal ones those in front: `count` pages, or all if there are no more. Pages that
  * the pool does not have are not chosen. chosen: int32 (B, Hkv, count), contiguous: the pages' places in the table's row, rising, and -1 behind.
- * first, last >= 0, first + last <= count. q, bounds: elem_dtype KVX_KV_BF16 / KVX_KV_F16; Hq / Hkv at most 16. workspace: kvx_paged_select_workspace_bytes(), contents do not
+ * first, last >= 0, first + last <= count. q, bounds: elem_dtype KVX_KV_BF16 / KVX_KV_F16; Hq / Hkv at most 16; B * Hkv below 2^21, and below 2^30 groups of 64 pages of them. workspace: kvx_paged_select_workspace_bytes(), contents do not
  * matter; calls that may overlap need one each. */
 typedef struct kvx_paged_select_args {
   int32_t num_pages, page_size, Hkv, D, elem_dtype, B, Hq, max_pages, count, first, last;
