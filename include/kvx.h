@@ -592,8 +592,8 @@ int kvx_paged_append(const kvx_paged_append_args* args, void* stream);
 /* Bounds of keys. For the pages that hold the last `tokens` of the first lens[b] tokens of every sequence (the same for all; shorter sequences: all of their pages):
  * the lowest and the highest of the page's keys among these lens[b], value by value, to bounds[page * b_stride_page + h * b_stride_h + d] and, b_stride_side further,
  * of the store's element type. Rows of codes count as kvx_paged_read gives them. A NaN among a page's values makes its bounds NaN. Bounds of other pages, and of pages
- * that the pool does not have, are left as they are. A page of two sequences gets the bounds of one of them: share pages that are full, or have as many tokens in
- * both. pages.v and the state of V are not read, but checked. lens and the table are read on the device alone. A call looks at fewer than 2^30 (sequence,
+ * that the pool does not have, are left as they are. A page of two sequences gets the bounds of one of them, or parts of each: share pages that are full, or have as
+ * many tokens in both. pages.v and the state of V are not read, but checked. lens and the table are read on the device alone. A call looks at fewer than 2^30 (sequence,
  * page, KV head), shorter sequences counted as the longest that the table and `tokens` allow. */
 typedef struct kvx_paged_bounds_args {
   kvx_pages pages;
@@ -612,8 +612,8 @@ int kvx_paged_bounds(const kvx_paged_bounds_args* args, void* stream);
  * not finite, or of bounds or queries that are not, counts as infinite. Of every (sequence, KV head)
  * the first `first` and the last `last` pages are chosen, and the others by their scores, of equal ones those in front: `count` pages, or all if there are no more. Pages that
  * the pool does not have are not chosen. chosen: int32 (B, Hkv, count), contiguous: the pages' places in the table's row, rising, and -1 behind.
- * first, last >= 0, first + last <= count. q, bounds: elem_dtype KVX_KV_BF16 / KVX_KV_F16; Hq / Hkv at most 16; B * Hkv below 2^21, and below 2^30 groups of 64 pages of them. workspace: kvx_paged_select_workspace_bytes(), contents do not
- * matter; calls that may overlap need one each. */
+ * first, last >= 0, first + last <= count <= 2^30. q, bounds: elem_dtype KVX_KV_BF16 / KVX_KV_F16; Hq / Hkv at most 16; B * Hkv below 2^21, and below 2^30 groups of
+ * 64 pages of them. workspace: kvx_paged_select_workspace_bytes(), contents do not matter; calls that may overlap need one each. */
 typedef struct kvx_paged_select_args {
   int32_t num_pages, page_size, Hkv, D, elem_dtype, B, Hq, max_pages, count, first, last;
   const void* q;

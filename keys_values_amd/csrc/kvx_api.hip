@@ -685,6 +685,7 @@ static int check_select(const kvx_paged_select_args* a) {
   KVX_REQUIRE(a->Hq / a->Hkv <= 16, KVX_ERR_UNSUPPORTED, "%s: %d query heads per KV head (at most 16)", who, a->Hq / a->Hkv);
   KVX_REQUIRE(a->count > 0 && a->first >= 0 && a->last >= 0 && (int64_t)a->first + a->last <= a->count, KVX_ERR_INVALID,
               "%s: count=%d must be positive, and first=%d and last=%d not negative and no more together", who, a->count, a->first, a->last);
+  KVX_REQUIRE(a->count <= (1 << 30), KVX_ERR_UNSUPPORTED, "%s: count=%d beyond 2^30", who, a->count);
   return KVX_OK;
 }
 

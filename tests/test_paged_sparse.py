@@ -154,7 +154,7 @@ def test_select_is_checked(kvx):
                 dict(block_table=0), dict(lens=0), dict(chosen=0), dict(bt_stride_b=-1)):
         assert _select(kvx, **bad) == INVALID, bad
     for bad in (dict(page_size=0), dict(page_size=8), dict(page_size=24), dict(page_size=2048), dict(D=96), dict(elem_dtype=_lib.KVX_KV_U8), dict(Hq=34), dict(Hkv=65536, Hq=65536),
-                dict(B=65536), dict(max_pages=2**26), dict(B=60000, Hkv=1000, Hq=1000)):
+                dict(B=65536), dict(max_pages=2**26), dict(B=60000, Hkv=1000, Hq=1000), dict(count=2**30 + 1), dict(count=2**31 - 1)):
         assert _select(kvx, **bad) == UNSUPPORTED, bad
 
 
