@@ -17,7 +17,7 @@ template <int D, int KV, bool INTERLEAVED, int U, bool PAST>  // PAST: queries p
 __global__ __launch_bounds__(512) void paged_append_kernel(const kvx_paged_append_args a, const int shift, const float factor, const int parts, const int stride,
                                                            const int64_t token_blocks, const int groups) {
   constexpr bool PLAIN = kv_is_plain(KV), U4 = kv_is_u4(KV), F16 = kv_elem_f16(KV);
-  constexpr int LPR = D / 8, ROWS = NTHREADS / LPR, ES = PLAIN ? 2 : 1;
+  constexpr int LPR = D / 8, ROWS = NTHREADS / LPR;
   const kvx_rotary_args& r = a.rotary;
   const kvx_pages& p = a.pages;
   const int col = threadIdx.x % LPR, mine = threadIdx.x / LPR, half = r.rotary_dim / 2, Hq = r.Hq, Hkv = r.Hkv;
