@@ -222,7 +222,8 @@ __device__ __forceinline__ uint32_t key_of(double sum) {
 
 struct SelectParams {
   kvx_paged_select_args a;
-  uint32_t* keys;  // (B, Hkv, max_pages)
+  uint32_t* keys;  // (B, Hkv, stride)
+  int stride;      // of tables' pages, in fours
   int shift;       // log2 of the page size
   int all_keys;    // few enough for all that a list has room for to be read, while its length is: 48 sequences of up to 8192 pages, 4 heads, 7.7 us, 8.4 without
   __device__ __forceinline__ int pages(int b) const { return (min(max(a.lens[b], 0), a.max_pages << shift) + a.page_size - 1) >> shift; }  // of a sequence
@@ -395,7 +396,7 @@ __global__ __launch_bounds__(NTHREADS, score_workgroups(D)) void select_score_ke
       const int h = (unit - begin_b) / units, from = unit - begin_b - h * units, count = min(units - from, end - unit), pair = b * Hkv + h;
       const typename S::template Fetch<NTHREADS> queries(a, b, h);
       const S s(a, qs, b, h, n, min(n, (from + count) * UNIT));
-      s.run(from * UNIT + wave * 16, UNIT, p.keys + (int64_t)pair * a.max_pages, [&] {
+      s.run(from * UNIT + wave * 16, UNIT, p.keys + (int64_t)pair * p.stride, [&] {
         if (again) __syncthreads();  // the queries before are read
         queries.put(qs);
         __syncthreads();
@@ -422,7 +423,7 @@ __global__ __launch_bounds__(4 * FEW) void select_few_kernel(const SelectParams 
   __shared__ __align__(16) typename S::Queries qs;
   __shared__ __align__(16) uint32_t keys[FEW];
   __shared__ int taken[FEW / 16];
-  const int pair = blockIdx.x, b = pair / a.Hkv, h = pair - b * a.Hkv, tid = threadIdx.x, lane = tid & 63;
+  const int b = blockIdx.y, h = blockIdx.x, pair = b * a.Hkv + h, tid = threadIdx.x, lane = tid & 63;
   const typename S::template Fetch<4 * FEW> queries(a, b, h);
   const int n = p.pages(b);
   if (tid < FEW) keys[tid] = kNever;
@@ -462,62 +463,87 @@ __global__ __launch_bounds__(4 * FEW) void select_few_kernel(const SelectParams 
   for (int j = all + tid; j < a.count; j += 4 * FEW) out[j] = -1;
 }
 
-// The `count` largest keys of a (sequence, KV head), of equal ones the first, in order of their pages, for up to R * NT pages, whose keys stay in registers. The last key that is taken lies
-// in one of 2048 equal parts of the keys' range, found by counting, then in one of 2048 parts of that, until no more of its part are left over (after three times a part is
+// The `count` largest keys of a (sequence, KV head), of equal ones the first, in order of their pages, for up to R * NT pages: R neighbours a lane, which stay in registers. The last key
+// that is taken lies in one of 2048 equal parts of a range of keys, found by counting, then in one of 2048 parts of that, until no more of its part are left over (after three times a part is
 // one key). By their upper bits instead, as the long form does, most keys would count in the same few places, one after the other.
 template <int R, int NT>
 __global__ __launch_bounds__(NT) void select_choose_kernel(const SelectParams p) {
   constexpr int BINS = 2048, WAVES = NT / 64, EACH = BINS / NT;  // EACH: parts a lane counts up, from the largest down
   const kvx_paged_select_args& a = p.a;
-  const int pair = blockIdx.x, b = pair / a.Hkv, n = p.pages(b), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  __shared__ int counts[BINS], sums[WAVES], at_bin, at_rest, at_count;
-  __shared__ uint32_t lows[WAVES], highs[WAVES];
-  __shared__ int places[R * WAVES];
-  const uint32_t* keys = p.keys + (int64_t)pair * a.max_pages;
+  const int b = blockIdx.y, pair = b * a.Hkv + blockIdx.x, n = p.pages(b), tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), first = R * tid;
+  __shared__ int counts[BINS], sums[WAVES], placed[WAVES], at_bin, at_rest, at_count;
+  __shared__ __align__(16) u32x4_t ranges[WAVES];
+  const uint32_t* keys = p.keys + (int64_t)pair * p.stride;
   int32_t* out = a.chosen + (int64_t)pair * a.count;
   uint32_t key[R];
+  constexpr int V = R < 4 ? R : 4;
+  typedef uint32_t Keys __attribute__((ext_vector_type(V)));
+  Keys x[R / V] = {};
+  if (p.all_keys) {  // does not wait for n
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-    if (r == 0 || p.all_keys) key[r] = keys[min(r * NT + tid, a.max_pages - 1)];  // does not wait for n
+    for (int v = 0; v < R / V; ++v) x[v] = *(const Keys*)(keys + min(first + V * v, p.stride - V));
+  } else {
 #pragma unroll
-  for (int r = 1; r < R; ++r)
-    if (!p.all_keys && r * NT < n) key[r] = keys[min(r * NT + tid, n - 1)];
+    for (int v = 0; v < R / V; ++v)
+      if (first + V * v < n) x[v] = *(const Keys*)(keys + first + V * v);
+  }
 #pragma unroll
-  for (int r = 0; r < R; ++r) key[r] = r * NT + tid < n ? key[r] : kNever;
+  for (int r = 0; r < R; ++r) key[r] = x[r / V][r % V];
 #pragma unroll
   for (int e = 0; e < EACH; ++e) counts[NT * e + tid] = 0;
   // ---- range of the keys that are neither taken anyway nor left out, and the numbers of those
   uint32_t low = kAlways, high = kNever;
-  int always = 0, others = 0;
+  uint32_t number = 0;  // those that are taken anyway << 16 | the others: of a workgroup at most R * NT in all, which is 32768
 #pragma unroll
   for (int r = 0; r < R; ++r) {
+    if (first + r >= n) key[r] = kNever;
     const bool other = key[r] != kNever && key[r] != kAlways;
-    if (other) {
-      low = min(low, key[r]);
-      high = max(high, key[r]);
-    }
-    always += __popcll(__ballot(key[r] == kAlways));
-    others += __popcll(__ballot(other));
+    low = other ? min(low, key[r]) : low;
+    high = other ? max(high, key[r]) : high;
+    number += key[r] == kAlways ? 1u << 16 : other ? 1u : 0u;
   }
-#pragma unroll
-  for (int step = 1; step < 64; step *= 2) {
-    low = min(low, (uint32_t)__shfl_xor((int)low, step, 64));
-    high = max(high, (uint32_t)__shfl_xor((int)high, step, 64));
-  }
-  if (lane == 0) {
-    lows[wave] = low;
-    highs[wave] = high;
-    sums[wave] = always << 16 | others;  // at most R * 64 each, which is 2048
-  }
+  // `least`: of the largest keys of groups of 2^levels lanes. With as many groups as keys are asked for, none below it is taken, and those need not be counted, which are most.
+  int levels = min(__builtin_clz(a.count) - __builtin_clz(n / R | 1), 6);
+  levels -= n / R >> max(levels, 0) < a.count;
+  uint32_t least = first < n ? high : kAlways;  // a group with lanes behind the last page says nothing
+  auto fold = [&](int level, auto ctrl, auto rows) {
+    auto other = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false); };
+    low = min(low, other(low));
+    high = max(high, other(high));
+    const uint32_t x = other(least);
+    least = level < levels ? max(least, x) : min(least, x);
+    number += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)number, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+  };
+  const std::integral_constant<int, 0xf> every;
+  auto fold_row = [&](int of, int lanes) {
+    fold(of, std::integral_constant<int, 0xB1>{}, every);       // quad_perm [1,0,3,2]
+    fold(of + 1, std::integral_constant<int, 0x4E>{}, every);   // quad_perm [2,3,0,1]
+    fold(of + 2, std::integral_constant<int, 0x141>{}, every);  // row_half_mirror
+    if (lanes == 16) fold(of + 3, std::integral_constant<int, 0x140>{}, every);  // row_mirror
+  };
+  fold_row(0, 16);
+  fold(4, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast:15 to the odd rows
+  fold(5, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast:31 to the upper half: lane 63 has all
+  if (lane == 63) ranges[wave] = u32x4_t{low, high, least, number};
   __syncthreads();
-  always = others = 0;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    low = min(low, lows[w]);
-    high = max(high, highs[w]);
-    always += sums[w] >> 16;
-    others += sums[w] & 0xffff;
-  }
+  const u32x4_t range = ranges[lane % WAVES];
+  low = range[0];
+  high = range[1];
+  least = range[2];
+  number = range[3];
+  fold_row(6, WAVES);
+  low = __builtin_amdgcn_readfirstlane(low);
+  high = __builtin_amdgcn_readfirstlane(high);
+  least = __builtin_amdgcn_readfirstlane(least);
+  number = __builtin_amdgcn_readfirstlane(number);
+  const int always = (int)(number >> 16), others = (int)(number & 0xffff);
+  // what the wavefronts in front of this one have, and all of them
+  auto over_waves = [&](const int* sums, uint32_t& all) {
+    const int x = lane < WAVES ? sums[lane] : 0, upto = scan(x);
+    all = (uint32_t)__builtin_amdgcn_readlane(upto, 63);
+    return (uint32_t)__builtin_amdgcn_readlane(upto - x, wave);
+  };
+  uint32_t all;
   // ---- `from`: the least key that is taken; `rest` of the keys equal to it, where there are more
   int rest = a.count - always;
   uint32_t from = low;
@@ -525,27 +551,26 @@ __global__ __launch_bounds__(NT) void select_choose_kernel(const SelectParams p)
   if (rest <= 0) {
     from = kAlways;
   } else if (others > rest) {
-    const int width = 32 - __builtin_clz((high - low) | 1u);
-    int shift = max(0, width - 11);
-    uint32_t to = high;  // the keys that are looked at: from .. to
+    if (levels >= 0 && least > low) from = least;  // 0 of a group that has no such key
+    uint32_t span = high - from;                   // keys from .. from + span are looked at
+    int shift = max(0, 21 - __builtin_clz(span | 1u));
     for (;;) {
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        if (key[r] >= from && key[r] <= to) atomicAdd(&counts[(key[r] - from) >> shift], 1);
+        if (key[r] - from <= span) atomicAdd(&counts[(key[r] - from) >> shift], 1);
       __syncthreads();
-      int c[EACH], all = 0;
+      int c[EACH], here = 0;
 #pragma unroll
       for (int e = 0; e < EACH; ++e) {
         c[e] = counts[BINS - 1 - EACH * tid - e];
-        all += c[e];
+        here += c[e];
       }
-      int upto = scan(all);
+      int upto = scan(here);
       if (lane == 63) sums[wave] = upto;
       __syncthreads();
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) upto += w < wave ? sums[w] : 0;
-      if (upto - all < rest && rest <= upto) {
-        int before = upto - all;
+      upto += (int)over_waves(sums, all);
+      if (upto - here < rest && rest <= upto) {
+        int before = upto - here;
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
           if (before < rest && rest <= before + c[e]) {
@@ -560,62 +585,45 @@ __global__ __launch_bounds__(NT) void select_choose_kernel(const SelectParams p)
       for (int e = 0; e < EACH; ++e) counts[BINS - 1 - EACH * tid - e] = 0;
       __syncthreads();
       rest = at_rest;
-      from += (uint32_t)at_bin << shift;
-      to = from + min((1u << shift) - 1, high - from);
+      const uint32_t skipped = (uint32_t)at_bin << shift;
+      from += skipped;
+      span = min((1u << shift) - 1, span - skipped);
       part = at_count > rest;
       if (!part || shift == 0) break;
       shift = max(0, shift - 11);
     }
   }
-  // ---- what is taken, in order
-  bool take[R];
+  // ---- what is taken, in order: keys above `from`, and the first of those equal to it
+  const uint32_t most = part ? rest : R * NT;
+  uint32_t above = 0, equal = 0;  // of the lane's keys
 #pragma unroll
-  for (int r = 0; r < R; ++r) take[r] = key[r] != kNever && key[r] >= from;
-  auto place = [&](const bool (&of)[R], int (&to)[R]) {  // places among those of all wavefronts and rows; returns how many there are
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const unsigned long long m = __ballot(of[r]);
-      to[r] = __popcll(m & ((1ull << lane) - 1));
-      if (lane == 0) places[r * WAVES + wave] = __popcll(m);
-    }
-    __syncthreads();
-    int before = 0, mine[R];
-    for (int first = 0; first < R * WAVES; first += 64) {
-      const int x = first + lane < R * WAVES ? places[first + lane] : 0, y = scan(x);
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (r * WAVES + wave >= first && r * WAVES + wave < first + 64) mine[r] = before + __shfl(y - x, r * WAVES + wave - first, 64);
-      before += __shfl(y, 63, 64);
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) to[r] += mine[r];
-    __syncthreads();
-    return before;
-  };
-  int to[R];
-  if (part) {
-    bool tie[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) tie[r] = key[r] == from;
-    place(tie, to);
-#pragma unroll
-    for (int r = 0; r < R; ++r) take[r] = take[r] && (key[r] != from || to[r] < rest);
+  for (int r = 0; r < R; ++r) {
+    above |= (uint32_t)(key[r] > from) << r;
+    equal |= (uint32_t)(key[r] == from) << r;
   }
-  const int taken = place(take, to);
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-    if (take[r] && to[r] < a.count) out[to[r]] = r * NT + tid;
-  for (int i = taken + tid; i < a.count; i += NT) out[i] = -1;
+  const uint32_t mine = __popc(above) | __popc(equal) << 16;  // of a workgroup no more than 32768 together
+  uint32_t before = scan((int)mine);
+  if (lane == 63) placed[wave] = (int)before;
+  __syncthreads();
+  before += over_waves(placed, all) - mine;
+  uint32_t ties = before >> 16, to = (before & 0xffff) + min(ties, most);
+  for (uint32_t left = above | equal; left; left &= left - 1) {
+    const int r = __builtin_ctz(left);
+    const bool tie = equal >> r & 1;
+    if ((!tie || ties < most) && to < (uint32_t)a.count) out[to++] = first + r;
+    ties += tie;
+  }
+  for (int i = (int)((all & 0xffff) + min(all >> 16, most)) + tid; i < a.count; i += NT) out[i] = -1;
 }
 
 // The same for any number of pages, whose keys are read again and again: the last key that is taken is found from its upper bits down, by counting.
 constexpr int CHOOSERS = 1024;
 __global__ __launch_bounds__(CHOOSERS) void select_choose_long_kernel(const SelectParams p) {
   const kvx_paged_select_args& a = p.a;
-  const int pair = blockIdx.x, b = pair / a.Hkv, n = p.pages(b), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.y, pair = b * a.Hkv + blockIdx.x, n = p.pages(b), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   constexpr int WAVES = CHOOSERS / 64, BINS = 2048;
   __shared__ int counts[BINS], sums[WAVES], at_bin, at_rest;
-  const uint32_t* keys = p.keys + (int64_t)pair * a.max_pages;
+  const uint32_t* keys = p.keys + (int64_t)pair * p.stride;
   int32_t* out = a.chosen + (int64_t)pair * a.count;
   // ---- the key of rank `count`: `rest` of those equal to it are taken
   uint32_t prefix = 0u;
@@ -710,20 +718,22 @@ int launch_paged_bounds(const kvx_paged_bounds_args& a, hipStream_t st) {
   return KVX_OK;
 }
 
-size_t paged_select_workspace(const kvx_paged_select_args& a) { return a.max_pages <= FEW ? 0 : (size_t)4 * a.B * a.Hkv * a.max_pages; }
+int keys_stride(const kvx_paged_select_args& a) { return (a.max_pages + 3) / 4 * 4; }
+size_t paged_select_workspace(const kvx_paged_select_args& a) { return a.max_pages <= FEW ? 0 : (size_t)4 * a.B * a.Hkv * keys_stride(a); }
 
 int launch_paged_select(const kvx_paged_select_args& a, hipStream_t st) {
-  const SelectParams p = {a, (uint32_t*)a.workspace, __builtin_ctz(a.page_size), (int64_t)a.B * a.Hkv * a.max_pages <= (1 << 21)};
+  const SelectParams p = {a, (uint32_t*)a.workspace, keys_stride(a), __builtin_ctz(a.page_size), (int64_t)a.B * a.Hkv * a.max_pages <= (1 << 21)};
   const int64_t count = (int64_t)a.B * a.Hkv, units = count * ((a.max_pages + UNIT - 1) / UNIT);
   KVX_REQUIRE(count < (1 << 21) && units < (1 << 30), KVX_ERR_UNSUPPORTED, "kvx_paged_select: %d sequences of up to %d pages, %d KV heads in one call", a.B, a.max_pages,
               a.Hkv);
   const unsigned blocks = (unsigned)min(units, (int64_t)score_workgroups(a.D) * num_cus());
   const int group = a.Hq / a.Hkv;
   const bool few = a.max_pages <= FEW;
+  const dim3 pairs(a.Hkv, a.B);
   auto go = [&](auto d, auto f16) {
     auto score = [&](auto heads) {
       constexpr int D = decltype(d)::value, HEADS = decltype(heads)::value;
-      if (few) hipLaunchKernelGGL((select_few_kernel<D, decltype(f16)::value, HEADS>), dim3((unsigned)count), dim3(4 * FEW), 0, st, p);
+      if (few) hipLaunchKernelGGL((select_few_kernel<D, decltype(f16)::value, HEADS>), pairs, dim3(4 * FEW), 0, st, p);
       else hipLaunchKernelGGL((select_score_kernel<D, decltype(f16)::value, HEADS>), dim3(blocks), dim3(NTHREADS), 0, st, p);
     };
     if (group <= 4) score(std::integral_constant<int, 1>{});
@@ -741,7 +751,6 @@ int launch_paged_select(const kvx_paged_select_args& a, hipStream_t st) {
     KVX_HIP(hipGetLastError());
     return KVX_OK;
   }
-  const dim3 pairs((unsigned)count);
   // 512 lanes take less time than 1024 up to 2048 pages, as long at 4096, and more beyond: 1024 pages 4.2 and 5.0 us, 4096 5.9 and 5.9, 8192 7.0 and 6.7
   auto choose = [&](auto r, auto nt) {
     constexpr int R = decltype(r)::value, NT = decltype(nt)::value;
