@@ -466,6 +466,9 @@ __global__ __launch_bounds__(4 * FEW) void select_few_kernel(const SelectParams 
 // The `count` largest keys of a (sequence, KV head), of equal ones the first, in order of their pages, for up to R * NT pages: R neighbours a lane, which stay in registers. The last key
 // that is taken lies in one of 2048 equal parts of a range of keys, found by counting, then in one of 2048 parts of that, until no more of its part are left over (after three times a part is
 // one key). By their upper bits instead, as the long form does, most keys would count in the same few places, one after the other.
+// What bounds it is that it runs once: a few workgroups fetch each of its instructions from afar, about 130 cycles for 64 bytes of them, more than the work itself takes. Hence one
+// order for all of a lane's keys, sums over wavefronts by lanes and not one after the other, a loop for the few that are taken: 8 lists of 8192 pages, 7.0 KB of code 6.6 us, 3.7 KB 5.3.
+// Keys that cannot be among the `count` largest kept from being counted (by the largest of groups of lanes): no gain.
 template <int R, int NT>
 __global__ __launch_bounds__(NT) void select_choose_kernel(const SelectParams p) {
   constexpr int BINS = 2048, WAVES = NT / 64, EACH = BINS / NT;  // EACH: parts a lane counts up, from the largest down
@@ -502,39 +505,31 @@ __global__ __launch_bounds__(NT) void select_choose_kernel(const SelectParams p)
     high = other ? max(high, key[r]) : high;
     number += key[r] == kAlways ? 1u << 16 : other ? 1u : 0u;
   }
-  // `least`: of the largest keys of groups of 2^levels lanes. With as many groups as keys are asked for, none below it is taken, and those need not be counted, which are most.
-  int levels = min(__builtin_clz(a.count) - __builtin_clz(n / R | 1), 6);
-  levels -= n / R >> max(levels, 0) < a.count;
-  uint32_t least = first < n ? high : kAlways;  // a group with lanes behind the last page says nothing
-  auto fold = [&](int level, auto ctrl, auto rows) {
+  auto fold = [&](auto ctrl, auto rows) {
     auto other = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false); };
     low = min(low, other(low));
     high = max(high, other(high));
-    const uint32_t x = other(least);
-    least = level < levels ? max(least, x) : min(least, x);
     number += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)number, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
   };
   const std::integral_constant<int, 0xf> every;
-  auto fold_row = [&](int of, int lanes) {
-    fold(of, std::integral_constant<int, 0xB1>{}, every);       // quad_perm [1,0,3,2]
-    fold(of + 1, std::integral_constant<int, 0x4E>{}, every);   // quad_perm [2,3,0,1]
-    fold(of + 2, std::integral_constant<int, 0x141>{}, every);  // row_half_mirror
-    if (lanes == 16) fold(of + 3, std::integral_constant<int, 0x140>{}, every);  // row_mirror
+  auto fold_row = [&](int lanes) {
+    fold(std::integral_constant<int, 0xB1>{}, every);   // quad_perm [1,0,3,2]
+    fold(std::integral_constant<int, 0x4E>{}, every);   // quad_perm [2,3,0,1]
+    fold(std::integral_constant<int, 0x141>{}, every);  // row_half_mirror
+    if (lanes == 16) fold(std::integral_constant<int, 0x140>{}, every);  // row_mirror
   };
-  fold_row(0, 16);
-  fold(4, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast:15 to the odd rows
-  fold(5, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast:31 to the upper half: lane 63 has all
-  if (lane == 63) ranges[wave] = u32x4_t{low, high, least, number};
+  fold_row(16);
+  fold(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast:15 to the odd rows
+  fold(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast:31 to the upper half: lane 63 has all
+  if (lane == 63) ranges[wave] = u32x4_t{low, high, number, 0u};
   __syncthreads();
   const u32x4_t range = ranges[lane % WAVES];
   low = range[0];
   high = range[1];
-  least = range[2];
-  number = range[3];
-  fold_row(6, WAVES);
+  number = range[2];
+  fold_row(WAVES);
   low = __builtin_amdgcn_readfirstlane(low);
   high = __builtin_amdgcn_readfirstlane(high);
-  least = __builtin_amdgcn_readfirstlane(least);
   number = __builtin_amdgcn_readfirstlane(number);
   const int always = (int)(number >> 16), others = (int)(number & 0xffff);
   // what the wavefronts in front of this one have, and all of them
@@ -551,7 +546,6 @@ __global__ __launch_bounds__(NT) void select_choose_kernel(const SelectParams p)
   if (rest <= 0) {
     from = kAlways;
   } else if (others > rest) {
-    if (levels >= 0 && least > low) from = least;  // 0 of a group that has no such key
     uint32_t span = high - from;                   // keys from .. from + span are looked at
     int shift = max(0, 21 - __builtin_clz(span | 1u));
     for (;;) {
@@ -751,7 +745,8 @@ int launch_paged_select(const kvx_paged_select_args& a, hipStream_t st) {
     KVX_HIP(hipGetLastError());
     return KVX_OK;
   }
-  // 512 lanes take less time than 1024 up to 2048 pages, as long at 4096, and more beyond: 1024 pages 4.2 and 5.0 us, 4096 5.9 and 5.9, 8192 7.0 and 6.7
+  // 512 lanes take less time than 1024 up to 4096 pages and more beyond: 1024 pages 4.2 and 5.0 us (with more code in both), 4096 5.0 and 5.2, 8192 5.4 and 5.2, 48 ragged
+  // lists of them 7.4 and 6.5
   auto choose = [&](auto r, auto nt) {
     constexpr int R = decltype(r)::value, NT = decltype(nt)::value;
     hipLaunchKernelGGL((select_choose_kernel<R, NT>), pairs, dim3(NT), 0, st, p);
@@ -761,7 +756,7 @@ int launch_paged_select(const kvx_paged_select_args& a, hipStream_t st) {
   if (a.max_pages <= 512) choose(std::integral_constant<int, 1>{}, half);
   else if (a.max_pages <= 1024) choose(std::integral_constant<int, 2>{}, half);
   else if (a.max_pages <= 2048) choose(std::integral_constant<int, 4>{}, half);
-  else if (a.max_pages <= 4096) choose(std::integral_constant<int, 4>{}, whole);
+  else if (a.max_pages <= 4096) choose(std::integral_constant<int, 8>{}, half);
   else if (a.max_pages <= 8192) choose(std::integral_constant<int, 8>{}, whole);
   else if (a.max_pages <= 16384) choose(std::integral_constant<int, 16>{}, whole);
   else if (a.max_pages <= 32768) choose(std::integral_constant<int, 32>{}, whole);
