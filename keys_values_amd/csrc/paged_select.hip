@@ -467,7 +467,7 @@ __global__ __launch_bounds__(4 * FEW) void select_few_kernel(const SelectParams 
 // that is taken lies in one of 2048 equal parts of a range of keys, found by counting, then in one of 2048 parts of that, until no more of its part are left over (after three times a part is
 // one key). By their upper bits instead, as the long form does, most keys would count in the same few places, one after the other.
 // What bounds it is that it runs once: a few workgroups fetch each of its instructions from afar, about 130 cycles for 64 bytes of them, more than the work itself takes. Hence one
-// order for all of a lane's keys, sums over wavefronts by lanes and not one after the other, a loop for the few that are taken: 8 lists of 8192 pages, 7.0 KB of code 6.6 us, 3.7 KB 5.3.
+// order for all of a lane's keys, sums over wavefronts by lanes and not one after the other, a loop for the few that are taken: 8 lists of 8192 pages, 7.0 KB of code 6.6 us, 3.3 KB 5.1.
 // Keys that cannot be among the `count` largest kept from being counted (by the largest of groups of lanes): no gain.
 template <int R, int NT>
 __global__ __launch_bounds__(NT) void select_choose_kernel(const SelectParams p) {

@@ -297,8 +297,8 @@ def test_select_of_batches(gpu, B, Hkv, low, high):
     gen = torch.Generator().manual_seed(B)
     lens = [high] + torch.randint(low, high + 1, (B - 1,), generator=gen).tolist()
     args = a_choice(gpu, lens, 4 * Hkv, Hkv, 64, 16, seed=B)
-    for count in (24, 500):
-        choose_and_check(*args, 16, count, 1, 2)
+    for count, first, last in ((24, 1, 2), (500, 1, 2), (24, 4, 20), (20, 20, 0), (3, 1, 1)):
+        choose_and_check(*args, 16, count, first, last)
 
 
 @pytest.mark.parametrize("width", [1, 2, 16, 17, 127, 128, 129, 512, 513, 1024, 1025, 2048, 2049, 4096, 4097, 8192, 8193, 16384, 16385, 32768, 32769])

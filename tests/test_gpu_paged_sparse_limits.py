@@ -38,7 +38,8 @@ def test_bounds_of_many_sequences(gpu, B, Hkv, D, page, tokens):
     assert torch.equal(bounds, want)
 
 
-@pytest.mark.parametrize("B,Hkv,group,width", [(65535, 2, 1, 3), (20000, 2, 4, 130), (9000, 5, 2, 128), (70, 1, 16, 600), (600, 2, 2, 2048), (300, 1, 4, 8200)])
+@pytest.mark.parametrize("B,Hkv,group,width", [(65535, 2, 1, 3), (20000, 2, 4, 130), (9000, 5, 2, 128), (70, 1, 16, 600), (1100, 2, 1, 1001), (600, 2, 2, 2048), (300, 2, 2, 4095),
+                                               (270, 1, 1, 8192), (300, 1, 4, 8200), (140, 1, 1, 16383), (70, 1, 2, 32767)])
 def test_select_of_many_sequences(gpu, B, Hkv, group, width):
     """Any sequences over a pool of few pages."""
     print("select", B, Hkv, group, width, flush=True)
