@@ -73,7 +73,7 @@ def check_append(qkv, got, want, Hq, D):
 @pytest.mark.parametrize("D,part", [(64, 64), (64, 16), (128, 128), (128, 48), (256, 256), (256, 32)])
 def test_append(gpu, D, part, store, interleaved, norm):
     print("append", D, part, store, interleaved, norm, flush=True)
-    for tokens, Hq, Hkv, page in ((1, 1, 1, 16), (37, 7, 1, 16), (70, 6, 3, 64), (5, 64, 8, 1024)):
+    for tokens, Hq, Hkv, page in ((1, 1, 1, 16), (37, 7, 1, 16), (70, 9, 3, 64), (5, 64, 8, 1024)):
         qkv, got, want, _ = append_both_ways(gpu, store, tokens, Hq, Hkv, D, page, part, interleaved, norm)
         check_append(qkv, got, want, Hq, D)
 
@@ -282,7 +282,7 @@ def test_select(gpu, D, dtype):
 
 @pytest.mark.parametrize("group", range(1, 17))
 def test_select_of_head_layouts(gpu, group):
-    for D, dtype, Hkv in ((64, torch.float16, 3), (128, torch.bfloat16, 1), (256, torch.bfloat16, 2)):
+    for D, dtype, Hkv in ((64, torch.float16, 5), (128, torch.bfloat16, 1), (256, torch.bfloat16, 2)):
         choose_and_check(*a_choice(gpu, [700, 0, 3000, 40], Hkv * group, Hkv, D, 16, dtype, seed=group), 16, 20)
 
 
@@ -487,8 +487,8 @@ def test_chosen_of_every_store(gpu, store, D):
 @pytest.mark.parametrize("group", [1, 2, 3, 5, 8, 12, 16])
 @pytest.mark.parametrize("store,D", [("bf16", 128), ("u8", 64), ("u4_fp16", 128), ("fp16", 256)])
 def test_chosen_of_head_layouts(gpu, store, D, group):
-    pool = Pool(gpu, store, [900, 0, 77], 3, D, 32, seed=group)
-    attend_and_check(pool, gpu, 3 * group, some_pages(pool, 6, seed=group))
+    pool = Pool(gpu, store, [900, 0, 77], 5, D, 32, seed=group)
+    attend_and_check(pool, gpu, 5 * group, some_pages(pool, 6, seed=group))
 
 
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256, 512, 1024])
