@@ -591,7 +591,7 @@ int kvx_paged_append(const kvx_paged_append_args* args, void* stream);
 
 /* Bounds of keys. For the pages that hold the last `tokens` of the first lens[b] tokens of every sequence (the same for all; shorter sequences: all of their pages):
  * the lowest and the highest of the page's keys among these lens[b], value by value, to bounds[page * b_stride_page + h * b_stride_h + d] and, b_stride_side further,
- * of the store's element type. Rows of codes count as kvx_paged_read gives them. A NaN among a page's values makes its bounds NaN. Bounds of other pages, and of pages
+ * of the store's element type. Rows of codes count as kvx_paged_read gives them, rounded to nearest: unrounded they may lie up to half a step outside. A NaN among a page's values makes its bounds NaN. Bounds of other pages, and of pages
  * that the pool does not have, are left as they are. A page of two sequences gets the bounds of one of them, or parts of each: share pages that are full, or have as
  * many tokens in both. pages.v and the state of V are not read, but checked. lens and the table are read on the device alone. A call looks at fewer than 2^30 (sequence,
  * page, KV head), shorter sequences counted as the longest that the table and `tokens` allow. */
@@ -608,8 +608,9 @@ int kvx_paged_bounds(const kvx_paged_bounds_args* args, void* stream);
 
 /* The pages that a query attends to. A page of a sequence (the i-th, i < ceil(lens[b] / page_size) and max_pages) has for KV head h the score
  *   max over the query heads of h of sum_d max(q[d] * low[d], q[d] * high[d]),
- * which, with bounds as kvx_paged_bounds leaves them (low <= high), is no less than any of its keys' products with them. Sums are formed in 64 bits and rounded to 32; a score that is
- * not finite, or of bounds or queries that are not, counts as infinite. Of every (sequence, KV head)
+ * which, with bounds as kvx_paged_bounds leaves them (low <= high), is no less than any of its keys' products with them, but for two roundings to nearest: the sum's, which is formed in 64 bits,
+ * to 32, and, of codes, the keys'. These count as kvx_paged_read gives them, while attention takes them unrounded: a product there may exceed the page's score by half a step of the
+ * element type (2^-8 of a bf16 value, 2^-11 of an fp16 one or 2^-25) of each of its terms. A score that is not finite, or of bounds or queries that are not, counts as infinite. Of every (sequence, KV head)
  * the first `first` and the last `last` pages are chosen, and the others by their scores, of equal ones those in front: `count` pages, or all if there are no more. Pages that
  * the pool does not have are not chosen. chosen: int32 (B, Hkv, count), contiguous: the pages' places in the table's row, rising, and -1 behind.
  * first, last >= 0, first + last <= count <= 2^30. q, bounds: elem_dtype KVX_KV_BF16 / KVX_KV_F16; Hq / Hkv at most 16; B * Hkv below 2^21, and below 2^30 groups of

@@ -1,6 +1,8 @@
 // Which pages of a sequence a query attends to, for gfx950: bounds of a page's keys, and the choice by what they allow.
 //   low, high = min, max over the page's keys, value by value (rows of codes: of the rows that they stand for, rounded to 16 bits);
-//   score = max over the query heads of a KV head of sum_d max(q_d low_d, q_d high_d) = sum_d (q+_d high_d + q-_d low_d), which no logit of the page exceeds.
+//   score = max over the query heads of a KV head of sum_d max(q_d low_d, q_d high_d) = sum_d (q+_d high_d + q-_d low_d),
+// which no product of the queries with the page's keys exceeds, codes' keys being those that are rounded (to nearest: bounds are what paged_read gives). Attention over codes takes them unrounded, and a
+// product there may be larger by 2^-8 (bf16; fp16 2^-11) of its sum of |q_d k_d|; in pages of one token about every second one is.
 #include <type_traits>
 
 #include "page_rows.h"

@@ -67,7 +67,7 @@ def paged_bounds(key_pages: torch.Tensor, bounds: torch.Tensor, block_table: tor
                  quant: Optional[ops.QuantState] = None) -> None:
     """Bring ``bounds`` (num_pages, n_query_groups, 2, head_size), of the rows' type, in line with the pages that hold the last ``tokens`` of the first
     ``lens`` tokens of every sequence (None: all of them): the lowest [.., 0, :] and the highest [.., 1, :] of the page's keys among these, value by value, of codes as
-    :func:`paged_read` gives their rows. A NaN among the keys makes a bound NaN. ``tokens`` is the most that any sequence has got since the last call: pages of
+    :func:`paged_read` gives their rows (rounded to nearest, so that the rows that attention takes may lie half a step outside). A NaN among the keys makes a bound NaN. ``tokens`` is the most that any sequence has got since the last call: pages of
     sequences that got fewer are looked at again, which changes nothing. Sequences that share a page should share it whole, or have as many tokens in it."""
     _lib.host().paged_bounds(key_pages, bounds, block_table, lens, tokens, quant)
 
