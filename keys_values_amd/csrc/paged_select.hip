@@ -232,7 +232,9 @@ struct SelectParams {
 };
 
 // v_mfma_f64_4x4x4, four blocks of 4 pages, 4 heads and 4 values: lane l has a value of page l % 16 (A), of head l % 4 (B), and gets the sum of page
-// 4 (l / 4 % 4) + l / 16 and head l % 4. Products of 16-bit values are exact in 32 bits, and their sums, in 64, differ with the order by less than what the rounding to 32 sees.
+// 4 (l / 4 % 4) + l / 16 and head l % 4. Products of 16-bit values are exact in 64 bits (bfloat16 ones go beyond the range of 32). The order of a page's sum is the same in every kernel, for every
+// split and place, so that the choice does not depend on these, and pages alike tie. In another order it may be off by D * 2^-53 of sum |q_d bound_d|, where the rounding to 32 bits sees 2^-24 of the
+// score: where large terms cancel the two orders round differently.
 // A wavefront takes 16 pages at a time and has the next 16 on their way meanwhile. Queries wait in LDS as pairs q+, q- of 64 bits, the 16 pairs of an instruction
 // side by side. An instruction takes 16 cycles (v_mfma_f64_16x16x4, four times as much work, a hundred).
 //
