@@ -608,11 +608,12 @@ int kvx_paged_bounds(const kvx_paged_bounds_args* args, void* stream);
 
 /* The pages that a query attends to. A page of a sequence (the i-th, i < ceil(lens[b] / page_size) and max_pages) has for KV head h the score
  *   max over the query heads of h of sum_d max(q[d] * low[d], q[d] * high[d]),
- * which, with bounds as kvx_paged_bounds leaves them (low <= high), is no less than any of its keys' products with them, but for two roundings to nearest: the sum's, which is formed in 64 bits,
- * to 32, and, of codes, the keys'. These count as kvx_paged_read gives them, while attention takes them unrounded: a product there may exceed the page's score by half a step of the
- * element type (2^-8 of a bf16 value, 2^-11 of an fp16 one or 2^-25) of each of its terms. A score that is not finite, or of bounds or queries that are not, counts as infinite. Of every (sequence, KV head)
- * the first `first` and the last `last` pages are chosen, and the others by their scores, of equal ones those in front: `count` pages, or all if there are no more. Pages that
- * the pool does not have are not chosen. chosen: int32 (B, Hkv, count), contiguous: the pages' places in the table's row, rising, and -1 behind.
+ * formed as sum_d (q+[d] * high[d] + q-[d] * low[d]), which is the same where low <= high; that is not checked. With bounds as kvx_paged_bounds leaves them it is no less than any of the
+ * keys' products with these heads, but for two roundings to nearest: the sum's, which is formed in 64 bits, to 32, and, of codes, the keys'. These count as kvx_paged_read gives them, while
+ * attention takes them unrounded: a product there may exceed the page's score by half a step of the element type (2^-8 of a bf16 value, 2^-11 of an fp16 one or 2^-25) in each of its terms.
+ * A score that is not finite, or of bounds or queries that are not, counts as infinite. Of every (sequence, KV head) the first `first` and the last `last` pages are chosen, and the others by
+ * their scores, of equal ones those in front: `count` pages, or all if there are no more. Pages that the pool does not have are not chosen. chosen: int32 (B, Hkv, count), contiguous: the
+ * pages' places in the table's row, rising, and -1 behind.
  * first, last >= 0, first + last <= count <= 2^30. q, bounds: elem_dtype KVX_KV_BF16 / KVX_KV_F16; Hq / Hkv at most 16; B * Hkv below 2^21, and below 2^30 groups of
  * 64 pages of them. workspace: kvx_paged_select_workspace_bytes(), contents do not matter; calls that may overlap need one each. */
 typedef struct kvx_paged_select_args {

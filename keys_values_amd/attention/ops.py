@@ -179,7 +179,7 @@ def paged_select(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.T
 
         max over the group's query heads of sum_d max(q[d] * lowest[d], q[d] * highest[d]),
 
-    of equal ones those in front. No key of a page has a larger product than this, but for roundings: of codes the bounds are those of the rows as ``kvcache.paged.paged_read`` rounds them, and
+    of equal ones those in front (formed as q+ * highest + q- * lowest, which is the same where lowest <= highest). No key of a page has a larger product than this, but for roundings: of codes the bounds are those of the rows as ``kvcache.paged.paged_read`` rounds them, and
     attention, which does not round them, may meet a product that is larger by half a step of the 16-bit type of each term. Sums are formed in 64 bits, in one order
     whatever the batch and however the work is split, and rounded to 32: pages alike tie; what is not finite counts as infinite. query (B, Hq, D); ``block_table`` (B, max_pages) and ``lens`` (B,) as for :func:`paged_decode`. Returns int32 (B, Hkv, count): places in the
     sequence's row of the table, rising, and -1 behind where it has fewer pages (all of them are chosen then). Pages that the pool does not have are

@@ -56,3 +56,17 @@ def test_pages_alike_tie_wherever_they_lie(gpu, D, dtype, group):
             more = torch.randint(1, (pages + 200) * page, (7,), generator=gen, dtype=torch.int32).to(gpu)
             more[-1] = lens[0]
             assert torch.equal(ops.paged_select(q.expand(7, -1, -1), bounds, wide, more, page, count, 0, 0)[-1], chosen[0])
+
+
+def test_bounds_the_wrong_way_round(gpu):
+    """Where a lowest value exceeds the highest, positive queries meet the second and negative ones the first all the same."""
+    gen = torch.Generator().manual_seed(3)
+    Hkv, group, D, pages, page = 2, 3, 64, 300, 16
+    q, bounds = torch.randn(1, Hkv * group, D, generator=gen).to(torch.bfloat16), torch.randn(pages, Hkv, 2, D, generator=gen).to(torch.bfloat16)
+    heads = q.double().view(Hkv, group, 1, D)
+    low, high = (bounds[:, :, i].transpose(0, 1)[:, None].double() for i in (0, 1))
+    score = (heads.clamp(min=0) * high + heads.clamp(max=0) * low).sum(-1).float().amax(1)
+    for n in (100, pages):
+        table, lens = torch.arange(n, dtype=torch.int32)[None].to(gpu), torch.tensor([n * page], dtype=torch.int32, device=gpu)
+        got = ops.paged_select(q.to(gpu), bounds.to(gpu), table, lens, page, 20, 0, 0)
+        assert torch.equal(got[0].cpu().long(), score[:, :n].sort(dim=-1, descending=True, stable=True).indices[:, :20].sort(-1).values)
