@@ -591,9 +591,9 @@ int kvx_paged_append(const kvx_paged_append_args* args, void* stream);
 
 /* Bounds of keys. For the pages that hold the last `tokens` of the first lens[b] tokens of every sequence (the same for all; shorter sequences: all of their pages):
  * the lowest and the highest of the page's keys among these lens[b], value by value, to bounds[page * b_stride_page + h * b_stride_h + d] and, b_stride_side further,
- * of the store's element type. Rows of codes count as kvx_paged_read gives them, rounded to nearest: unrounded they may lie up to half a step outside. A NaN among a page's values makes its bounds NaN. Bounds of other pages, and of pages
- * that the pool does not have, are left as they are. A page of two sequences gets the bounds of one of them, or parts of each: share pages that are full, or have as
- * many tokens in both. pages.v and the state of V are not read, but checked. lens and the table are read on the device alone. A call looks at fewer than 2^30 (sequence,
+ * of the store's element type. Rows of codes count as kvx_paged_read gives them, rounded to nearest: unrounded they may lie up to half a step outside. A NaN among a page's values
+ * makes its bounds NaN. Bounds of other pages, and of pages that the pool does not have, are left as they are. A page of two sequences gets the bounds of one of them, or parts of each:
+ * share pages that are full, or have as many tokens in both; a sequence with several new tokens is given once, with the last one's length. pages.v and the state of V are not read, but checked. lens and the table are read on the device alone. A call looks at fewer than 2^30 (sequence,
  * page, KV head), shorter sequences counted as the longest that the table and `tokens` allow. */
 typedef struct kvx_paged_bounds_args {
   kvx_pages pages;

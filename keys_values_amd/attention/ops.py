@@ -183,7 +183,8 @@ def paged_select(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.T
     attention, which does not round them, may meet a product that is larger by half a step of the 16-bit type of each term. Sums are formed in 64 bits, in one order
     whatever the batch and however the work is split, and rounded to 32: pages alike tie; what is not finite counts as infinite. query (B, Hq, D); ``block_table`` (B, max_pages) and ``lens`` (B,) as for :func:`paged_decode`. Returns int32 (B, Hkv, count): places in the
     sequence's row of the table, rising, and -1 behind where it has fewer pages (all of them are chosen then). Pages that the pool does not have are
-    not chosen. ``last`` of 1 or more keeps the page that the new token has been written to."""
+    not chosen. ``last`` of 1 or more keeps the page that the new token has been written to. Several new tokens of a
+    sequence: its row of the table once for each, with lengths of their own; the bounds of a page that later ones lie in too allow more than the earlier ones see."""
     return _lib.host().paged_select(query, bounds, block_table, lens, page_size, count, first, last)
 
 

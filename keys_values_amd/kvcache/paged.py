@@ -20,7 +20,8 @@ an earlier one had its workspace). There is no CPU path.
 Long sequences need not be read whole for a token. With the lowest and the highest of each page's keys at hand (``paged_bounds``, twice a row's bytes a page),
 ``attention.ops.paged_select`` finds the pages that can matter to a query, and ``attention.ops.paged_decode_chosen`` attends to those. A layer's step is
 then ``paged_append`` (rotation and write in one launch), ``paged_bounds`` of the page written to (``tokens=1``), ``paged_select``, ``paged_decode_chosen``; a pool made
-with ``bounds=True`` has them as methods.
+with ``bounds=True`` has them as methods. Several new tokens of a sequence: one append, one ``paged_bounds`` with the sequence's new length and ``tokens`` their number, then the
+row of the table once a token, with the token's own length, in the other two.
 """
 from typing import Optional, Tuple
 
@@ -67,8 +68,10 @@ def paged_bounds(key_pages: torch.Tensor, bounds: torch.Tensor, block_table: tor
                  quant: Optional[ops.QuantState] = None) -> None:
     """Bring ``bounds`` (num_pages, n_query_groups, 2, head_size), of the rows' type, in line with the pages that hold the last ``tokens`` of the first
     ``lens`` tokens of every sequence (None: all of them): the lowest [.., 0, :] and the highest [.., 1, :] of the page's keys among these, value by value, of codes as
-    :func:`paged_read` gives their rows (rounded to nearest, so that the rows that attention takes may lie half a step outside). A NaN among the keys makes a bound NaN. ``tokens`` is the most that any sequence has got since the last call: pages of
-    sequences that got fewer are looked at again, which changes nothing. Sequences that share a page should share it whole, or have as many tokens in it."""
+    :func:`paged_read` gives their rows (rounded to nearest, so that the rows that attention takes may lie half a step outside). A NaN among the keys makes a bound NaN.
+    ``tokens`` is the most that any sequence has got since the last call: pages of sequences that got fewer are looked at again, which changes nothing. Sequences that share a
+    page should share it whole, or have as many tokens in it: where they have not, its bounds are one's or parts of each. A sequence with several new tokens is given once, with
+    all of them counted, also where ``attention.ops.paged_select`` is then given its row of the table once a token: a page's bounds hold for any of its tokens."""
     _lib.host().paged_bounds(key_pages, bounds, block_table, lens, tokens, quant)
 
 
