@@ -226,13 +226,15 @@ template <typename T>
 __device__ __forceinline__ T once(const void* p) { return __builtin_nontemporal_load((const T*)p); }
 
 // Wavefronts a SIMD that the registers have to leave room for. Plain rows of 256 values take more than half of them. Plain rows of 128 fit a third wavefront only if
-// asked to, which short pairs gain from (256 sequences of 50 to 400 tokens, 32 / 8 heads: 49.1 us with two, 42.8 with three). No bound here spills.
-constexpr int waves_per_simd(int D, bool codes) { return D == 256 && !codes ? 1 : D == 128 && !codes ? 3 : 2; }
+// asked to, which short pairs gain from (256 sequences of 50 to 400 tokens, 32 / 8 heads: 49.1 us with two, 42.8 with three). Over chosen pages they hold more and would spill
+// five registers for a third one: two there (64 sequences of 20000 tokens, 64 pages of 16: 51.3 us with three, 48.5 with two; 2 sequences 7.3 and 6.8; 8 of 60000, 256
+// pages of 64: 106 and 104). No bound here spills vector registers.
+constexpr int waves_per_simd(int D, bool codes, bool chosen) { return D == 256 && !codes ? 1 : D == 128 && !codes && !chosen ? 3 : 2; }
 
 // CHOSEN: over the pages that a list names, of a (sequence, KV head) its own. A key's place in the pair is that in the list's pages then, one behind the other, and its place
 // in the sequence, which says whether there is such a token, comes of the list's entry: 16 keys are in one page, and `live` of them are tokens.
 template <int D, int KV, bool CHOSEN>
-__global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV))) void paged_decode_kernel(const std::conditional_t<CHOSEN, ChosenParams, PagedParams> p) {
+__global__ __launch_bounds__(NT, waves_per_simd(D, !kv_is_plain(KV), CHOSEN)) void paged_decode_kernel(const std::conditional_t<CHOSEN, ChosenParams, PagedParams> p) {
   using R = Rows<D, KV>;
   constexpr bool F16 = R::F16, CODES = R::CODES, U4 = R::U4, P16 = F16 || CODES;  // P16: weights and operands in fp16
   constexpr int KJ = R::KJ, DPL = R::DPL, ES = R::ES;
@@ -875,8 +877,10 @@ ChosenParams params_of(const kvx_paged_decode_args& a, const kvx_chosen_pages* c
   p.cus = num_cus();
   // One workgroup a compute unit for the only pair: the partials of more take longer to join than they save (one of 100000 tokens, 16 heads of 128: 21.7 us, 33.8
   // with three).
-  // More of them than registers leave room for would come in a second round: 239 sequences of 1 to 641, 24 / 8 heads of 128, 8-bit: 28.7, 35.7 with three.
-  const int64_t per_cu = g.D == 256 ? waves_per_simd(256, !plain) : g.D == 128 && !plain && !kv_is_u4(g.kv_dtype) ? 2 : 3;
+  // More of them than registers leave room for would come in a second round: 239 sequences of 1 to 641, 24 / 8 heads of 128, 8-bit: 28.7, 35.7 with three; whole lists of
+  // plain rows of 128 (256 sequences of 300 to 3000, 64 pages of 16, 28 / 4 heads): 93.8, 98.8 with three. Lists in parts take as long with either.
+  const bool two = plain ? c && p.whole : !kv_is_u4(g.kv_dtype);
+  const int64_t per_cu = g.D == 256 ? waves_per_simd(256, !plain, c) : g.D == 128 && two ? 2 : 3;
   const int64_t pairs = (int64_t)a.B * a.pages.Hkv, units = pairs * ((p.cap + (1 << p.unit) - 1) >> p.unit), most = p.cus * (pairs < per_cu ? pairs : per_cu);
   p.workgroups = (int)(units < most ? units : most);
   p.by_pair = pairs <= p.workgroups;
