@@ -144,6 +144,8 @@ int launch_paged_append(const kvx_paged_append_args& a, hipStream_t st) {
   const int64_t each = NTHREADS / lpr, groups = (r.tokens + each - 1) / each, lanes = (int64_t)heads * lpr;
   // A token's rows over several workgroups where few tokens leave units idle; over one, up to three a lane, where more tokens would read the angles again.
   const int parts = r.tokens <= 2 * num_cus() ? (int)((lanes + NTHREADS - 1) / NTHREADS) : 1;
+  // Lanes of a token are few hundreds; 18705 tokens of plain rows of 128, us with one, two and three rows a lane: 8 / 2 heads (192 lanes) 21.8, 26.3, 25.3; 16 / 4 (384) 52.4, 43.9, 44.1; 32 / 8
+  // (768) 98, 88, 81. In between, 28 / 4 (576) 83, 69, 62 and 24 / 8 (640) 86, 73, 68, three would do better than the two that they take; queries of pages of codes (32 / 8, 512) 89, 87, 93.
   const int u = parts > 1 || lanes <= NTHREADS ? 1 : lanes <= 640 ? 2 : 3;
   const int threads = parts > 1 || !plain ? NTHREADS : (int)min((lanes + 64 * u - 1) / (64 * u) * 64, (int64_t)512), stride = parts * u * (threads / lpr);
   const bool past = r.tokens * lanes * 16 > (64ll << 20);

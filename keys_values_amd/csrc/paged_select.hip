@@ -39,6 +39,9 @@ __device__ __forceinline__ void fold_rows(float (&x)[N], F best) {  // of x[0 ..
 // not have: all loads of a step are on their way before the first is waited for.
 // 142000 tokens in pages of 16, 8 heads of 128 (290 MB of keys, 37 of bounds): 64 us, with loads through the caches 71. A grid of all pages that the tables have room for takes 63
 // there, but longer the emptier the tables are.
+// W goes by the page's size, 1 up to 32, 4 up to 128, 16 above (same tokens, us with 1, 4 and 16): pages of 32 60, 68, 291; 64 63, 61, 154; 128 60, 61, 86; 256 60 with any; 1024 66, 60, 62.
+// Of the newest page of 32 sequences alone: 64 3.8, 3.4, 5.1; 256 6.3, 5.5, 5.2; 1024 38.9, 14.3, 13.0. Pages of codes, which have less to load, would take fewer: 8-bit
+// pages of 64 40.5, 45.7, 186; of 256 35.3, 34.2, 54.
 template <int D, int KV, int W>
 __global__ __launch_bounds__(W == 16 ? 1024 : 256) void paged_bounds_kernel(const kvx_paged_bounds_args a, const int shift) {
   constexpr bool PLAIN = kv_is_plain(KV), U4 = kv_is_u4(KV), F16 = kv_elem_f16(KV);
@@ -358,7 +361,9 @@ struct Scorer {
   }
 };
 
-constexpr int score_workgroups(int D) { return D == 256 ? 2 : 4; }  // a compute unit: what registers leave room for
+// Workgroups a compute unit. Registers leave room for four with rows of 128, two with rows of 256 and more than four heads a group; elsewhere for more, which would take a little less: rows of 64
+// (16 sequences of 131072 in pages of 32, 32 / 8 heads) 34.3 us with six, 35.4 with four; rows of 256 and up to four heads (4 such sequences) 35.3 with three, 36.3 with two.
+constexpr int score_workgroups(int D) { return D == 256 ? 2 : 4; }
 template <int D, bool F16, int HEADS /* of the group, in fours */>
 __global__ __launch_bounds__(NTHREADS, score_workgroups(D)) void select_score_kernel(const SelectParams p) {
   typedef Scorer<D, F16, HEADS> S;
@@ -614,7 +619,8 @@ __global__ __launch_bounds__(NT) void select_choose_kernel(const SelectParams p)
   for (int i = (int)((all & 0xffff) + min(all >> 16, most)) + tid; i < a.count; i += NT) out[i] = -1;
 }
 
-// The same for any number of pages, whose keys are read again and again: the last key that is taken is found from its upper bits down, by counting.
+// The same for any number of pages, whose keys are read again and again: the last key that is taken is found from its upper bits down, by counting. Slow: most keys count in the same few
+// places, and each 1024 pages wait four times in the last pass. 65536 pages, one list or eight, 138 us (their scores 12 and 67), 131072 248 and 271; 32768 pages by the kernel above 12.
 constexpr int CHOOSERS = 1024;
 __global__ __launch_bounds__(CHOOSERS) void select_choose_long_kernel(const SelectParams p) {
   const kvx_paged_select_args& a = p.a;
