@@ -865,8 +865,9 @@ ChosenParams params_of(const kvx_paged_decode_args& a, const kvx_chosen_pages* c
   // Tables of up to 512 tokens: a pair is a workgroup's, and there is no second launch.
   p.unit = p.cap <= 4 * UNIT ? 9 : 7;
   // Lists of pages are mostly full, so that pairs have as much work each: where they are enough to keep the units busy, a list of up to 2048 tokens is a workgroup's too. 64 pages of
-  // 16, 32 / 8 heads of 128, kernel and join or kernel alone: 24 sequences, plain 28.4 and 24.1 us, 32 32.7 and 27.9, 64 56.2 and 51.4, 8-bit 32 26.2 and 20.0; but 8
-  // sequences, plain, 16.6 and 19.8. Where most sequences have few tokens the longest list takes longer than it would in parts (1024 plain keys 20 us, 13 and 4 in parts).
+  // 16, 32 / 8 heads of 128, kernel and join or kernel alone: 24 sequences, plain 21.7 + 4 and 22.0 us, 32 29.9 + 4.7 and 29.6, 64 56 + 4.5 and 56, 8-bit 32 22 + 4.4 and 19.7; but 8
+  // sequences, plain, 10.9 + 4.1 and 18.8. The lengths are not known here: where most sequences are shorter than their lists (even in the logarithm from 1 to 1500), 64 take 19.5 + 4 and
+  // 21.3, but 256 61 + 4.7 and 78.
   const int64_t lists = (int64_t)a.B * g.Hkv;
   if (c && p.cap > 4 * UNIT && p.cap <= 2048 && 4 * lists >= p.cap) p.unit = 32 - __builtin_clz(p.cap - 1);
   p.whole = !splits(p);
